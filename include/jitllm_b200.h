@@ -278,6 +278,110 @@ int32_t jl_gemv_argmax_static(int32_t ggml_type, int64_t rows, int64_t cols, con
 int32_t jl_static_status(void *stream);
 const char *jl_static_last_error(void);
 
+/* ---- 8-bit paged key/value cache on device buffers of the caller (no counterpart in the reference, whose pages are binary16
+ * or binary32: runtime/kv/KvStorageRequest.java:5-12). Three operators that follow one another in a step:
+ *   jl_kv8_map        sequence lengths -> block table, and place, position and sequence of every new token, all on the GPU
+ *                     (the host-side steps of runtime/kv/BlockPool.java and of jl_kv_publish_block_table);
+ *   jl_kv8_append     keys (rotated on the way, if asked) and values of new tokens -> 8-bit codes with a scale per token and head;
+ *   jl_kv8_attention  attention of single tokens over the pages, with the rotation of the queries.
+ * All pointers in the argument structures are device pointers on the context's GPU. Every call is enqueued on `stream` (a
+ * cudaStream_t of that GPU; NULL is the default stream, jl_stream(ctx) the context's own) and returns without waiting; none
+ * allocates or synchronises, so all may be captured into CUDA graphs. The argument structure is read during the call only.
+ * What the device finds wrong (an index beyond its bounds) is passed over as described at each field; it never leads to an
+ * access outside the buffers described. The current device is left as it was. */
+
+/* Pages. Block b of keys (values) starts block_stride bytes (elements) behind block b - 1 and holds
+ * int8 [kv_heads][block_tokens][head_dim]; its scales start scale_stride floats behind those of block b - 1 and are
+ * float [kv_heads][block_tokens]. An element's value is code * scale. Strides beyond one block interleave the layers of a model.
+ * k and v 16-byte aligned, block_stride a multiple of 16 and at least kv_heads * block_tokens * head_dim, scale_stride at
+ * least kv_heads * block_tokens; head_dim 64, 96, 128, 192 or 256; block_tokens 1..65536; kv_heads 1..1024. */
+typedef struct {
+    int8_t *k, *v;
+    float *k_scale, *v_scale;
+    int64_t block_stride, scale_stride;
+    int32_t blocks, block_tokens, kv_heads, head_dim;
+} jl_kv8_pages;
+
+/* Device memory that jl_kv8_map and jl_kv8_attention keep their partial results and arrival counters in: about 10 MB, made once.
+ * Calls with one workspace must not overlap on the GPU: one workspace for each stream (or captured graph) that runs beside
+ * others. Calls of any shape may follow one another. Free it when no call with it is under way and no graph holds one. */
+typedef struct jl_kv8_workspace jl_kv8_workspace;
+int32_t jl_kv8_workspace_create(jl_ctx *ctx, jl_kv8_workspace **out);
+int32_t jl_kv8_workspace_free(jl_ctx *ctx, jl_kv8_workspace *ws);
+
+/* Block table and slot map. Sequence r holds held[r] tokens and gets added[r] more. Sequences are served in order: one whose
+ * tokens need new blocks takes them from free_blocks, from *cursor on, and their ids follow the ids of its blocks in its row of
+ * the table; the table's other entries are left as they are. A sequence is refused (nothing of it changes, its tokens get
+ * position and place -1) if held or added is negative, if it would grow beyond blocks_per_slot blocks, if its tokens do not all
+ * lie within `capacity`, or if the blocks it needs, together with those that the sequences before it need (refused for lack of
+ * blocks or not), are more than there are.
+ * New tokens are numbered through, sequence after sequence: token offsets[r] + i is sequence r's token at position held[r] + i
+ * and belongs at place block * block_tokens + position % block_tokens of the pages (-1 where the table holds no block >= 0).
+ * Entries of the token arrays from the last token on are left as they are. */
+typedef struct {
+    const int32_t *held, *added;    /* [sequences] */
+    const int32_t *free_blocks;     /* [free_count] ids of free blocks; may be NULL if free_count is 0 */
+    const int32_t *cursor;          /* [1] how many of them are taken already; outside 0..free_count: none is left */
+    int32_t *cursor_out;            /* [1] the same after this call; may be `cursor` */
+    int32_t *block_table;           /* [sequences][blocks_per_slot] */
+    int32_t *lengths;               /* [sequences] tokens held after this call; may be `held` */
+    int32_t *offsets;               /* [sequences + 1] or NULL: number of the first new token; at most 2^31 - 1 */
+    int32_t *token_slots;           /* [capacity] or NULL: the token's sequence */
+    int32_t *positions;             /* [capacity] or NULL */
+    int64_t *slot_map;              /* [capacity] */
+    int32_t *result;                /* [4]: new tokens (at most capacity), blocks taken, sequences refused, blocks asked for */
+    int32_t sequences;              /* 1..8192 */
+    int32_t blocks_per_slot, block_tokens, free_count, capacity;
+} jl_kv8_map_args;
+int32_t jl_kv8_map(jl_ctx *ctx, jl_kv8_workspace *ws, const jl_kv8_map_args *args, void *stream);
+
+/* Append. Row t of k and v is [kv_heads][head_dim], row strides in elements. With rope_cos / rope_sin (tables of jl_upload_rope,
+ * [rope_rows][head_dim / 2]) pairs (2i, 2i + 1) of the keys are rotated by the angle of positions[t] first. Then, for each token
+ * and head, scale = max |x| / 127 and code = x / scale rounded to the nearest (ties to even), as if computed without rounding
+ * before; a row whose largest element is below 2^-100 is stored as zeros, one with an infinite or NaN element with a NaN scale and
+ * codes 0, and so are the keys of a token whose position is outside the tables. Rows with a place outside the pages (such as
+ * -1), and rows from *token_count on, are not stored. Places of one call have to differ. */
+typedef struct {
+    jl_kv8_pages pages;
+    const void *k, *v;              /* [tokens], 16-byte aligned; strides multiples of 16 bytes and at least kv_heads * head_dim */
+    int64_t k_stride, v_stride;
+    const int64_t *slot_map;        /* [tokens] */
+    const int32_t *positions;       /* [tokens]; NULL without rope tables */
+    const float *rope_cos, *rope_sin;  /* both or neither */
+    const int32_t *token_count;     /* [1] or NULL: how many of the rows are tokens (result[0] of jl_kv8_map) */
+    int32_t tokens, rope_rows;
+    int32_t ggml_type;              /* of k and v: JL_F32 or JL_F16 */
+} jl_kv8_append_args;
+int32_t jl_kv8_append(jl_ctx *ctx, const jl_kv8_append_args *args, void *stream);
+
+/* Attention. Row r's queries [heads][head_dim] (query head h reads KV head h / (heads / kv_heads)) attend to the tokens
+ * 0 .. positions[r] of sequence kv_slots[r], or to the last `window` of these: out = sum softmax(scale * q.k) v,
+ * lse = ln sum exp(scale * q.k). Queries are rotated like the keys of jl_kv8_append if rope tables are given (a position
+ * beyond them makes the row NaN). Tokens beyond the table's row, and tokens whose table entry is no block of the pages, have no
+ * weight. A row that attends to nothing (position -1, a sequence outside 0..slots - 1) gets zeros and lse -inf; rows from
+ * *token_count on are left as they are. A NaN scale, query or key makes NaN of the outputs that it has weight in. */
+typedef struct {
+    jl_kv8_pages pages;
+    const void *q;                  /* [rows], 16-byte aligned, row stride in elements a multiple of 16 bytes */
+    void *out;                      /* [rows], as q */
+    float *lse;                     /* [rows][heads] or NULL */
+    int64_t q_stride, out_stride;
+    const int32_t *block_table;     /* [slots][blocks_per_slot] */
+    const int32_t *kv_slots;        /* [rows] or NULL: row r is sequence r */
+    const int32_t *positions;       /* [rows] */
+    const float *rope_cos, *rope_sin;  /* both or neither */
+    const int32_t *token_count;     /* [1] or NULL */
+    int32_t rows, heads, slots, blocks_per_slot;
+    int32_t window;                 /* 0: all tokens */
+    int32_t rope_rows;
+    int32_t ggml_type;              /* of q and out: JL_F32 or JL_F16 */
+    float scale;
+} jl_kv8_attention_args;
+int32_t jl_kv8_attention(jl_ctx *ctx, jl_kv8_workspace *ws, const jl_kv8_attention_args *args, void *stream);
+/* The checks of arguments that the three calls make before anything else (which: 0 = map, 1 = append, 2 = attention), with
+ * their message; needs no GPU. */
+int32_t jl_debug_kv8_check(int32_t which, const void *args, char *message, size_t n);
+
 #ifdef __cplusplus
 }
 #endif

@@ -26,3 +26,4 @@ from .api import (  # noqa: F401
 )
 from .tensor_parallel import TensorParallel, local_shape, shard_tensor, torch_broadcast  # noqa: F401,E402
 from .gguf import GgufFile, load_model_gguf, write_gguf  # noqa: F401,E402
+from .kv8 import Kv8Append, Kv8Attention, Kv8Map, Kv8Pages, Kv8Workspace  # noqa: F401,E402

@@ -31,6 +31,42 @@ class JlCounters(C.Structure):
     ]
 
 
+class JlKv8Pages(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("block_stride", C.c_int64), ("scale_stride", C.c_int64),
+        ("blocks", C.c_int32), ("block_tokens", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+    ]
+
+
+class JlKv8MapArgs(C.Structure):
+    _fields_ = [
+        ("held", C.c_void_p), ("added", C.c_void_p), ("free_blocks", C.c_void_p), ("cursor", C.c_void_p),
+        ("cursor_out", C.c_void_p), ("block_table", C.c_void_p), ("lengths", C.c_void_p), ("offsets", C.c_void_p),
+        ("token_slots", C.c_void_p), ("positions", C.c_void_p), ("slot_map", C.c_void_p), ("result", C.c_void_p),
+        ("sequences", C.c_int32), ("blocks_per_slot", C.c_int32), ("block_tokens", C.c_int32),
+        ("free_count", C.c_int32), ("capacity", C.c_int32),
+    ]
+
+
+class JlKv8AppendArgs(C.Structure):
+    _fields_ = [
+        ("pages", JlKv8Pages), ("k", C.c_void_p), ("v", C.c_void_p), ("k_stride", C.c_int64), ("v_stride", C.c_int64),
+        ("slot_map", C.c_void_p), ("positions", C.c_void_p), ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p),
+        ("token_count", C.c_void_p), ("tokens", C.c_int32), ("rope_rows", C.c_int32), ("ggml_type", C.c_int32),
+    ]
+
+
+class JlKv8AttentionArgs(C.Structure):
+    _fields_ = [
+        ("pages", JlKv8Pages), ("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p),
+        ("q_stride", C.c_int64), ("out_stride", C.c_int64), ("block_table", C.c_void_p), ("kv_slots", C.c_void_p),
+        ("positions", C.c_void_p), ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p), ("token_count", C.c_void_p),
+        ("rows", C.c_int32), ("heads", C.c_int32), ("slots", C.c_int32), ("blocks_per_slot", C.c_int32),
+        ("window", C.c_int32), ("rope_rows", C.c_int32), ("ggml_type", C.c_int32), ("scale", C.c_float),
+    ]
+
+
 _P = C.c_void_p
 _I32 = C.c_int32
 _I64 = C.c_int64
@@ -85,6 +121,12 @@ SIGNATURES = {
     "jl_gguf_upload": (_I32, [_P, _P, _I32, _I32, _I32, _P, _P, C.c_int64]),
     "jl_gguf_close": (None, [_P]),
     "jl_gguf_last_error": (C.c_char_p, []),
+    "jl_kv8_workspace_create": (_I32, [_P, C.POINTER(_P)]),
+    "jl_kv8_workspace_free": (_I32, [_P, _P]),
+    "jl_debug_kv8_check": (_I32, [_I32, _P, C.c_char_p, C.c_size_t]),
+    "jl_kv8_map": (_I32, [_P, _P, C.POINTER(JlKv8MapArgs), _P]),
+    "jl_kv8_append": (_I32, [_P, C.POINTER(JlKv8AppendArgs), _P]),
+    "jl_kv8_attention": (_I32, [_P, _P, C.POINTER(JlKv8AttentionArgs), _P]),
 }
 
 _lib = None

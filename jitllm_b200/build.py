@@ -21,7 +21,7 @@ CSRC = PKG / "csrc"
 LIB = PKG / "lib"
 
 CUDA_SOURCES = ["gemv.cu", "ops.cu", "attn_split.cu", "engine.cu", "static_entry.cu", "gemm_tc.cu", "gemm_wide.cu", "attn_prompt_tc.cu", "tp_exchange.cu", "gguf_loader.cu",
-                "sampler.cu"]
+                "sampler.cu", "kv8.cu", "kv8_checks.cu", "kv8_attention.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",

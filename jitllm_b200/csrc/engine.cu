@@ -13,6 +13,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <map>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -21,6 +22,7 @@
 #include "sampler.cuh"
 #include "gemm_tc.cuh"
 #include "tp_exchange.cuh"
+#include "kv8.cuh"
 
 #include <unistd.h>
 
@@ -62,6 +64,10 @@ struct StepGraph {
 
 struct jl_tensor {
     DevTensor t;
+};
+
+struct jl_kv8_workspace {
+    Kv8Scratch scratch;
 };
 
 struct jl_ctx {
@@ -143,6 +149,7 @@ struct jl_ctx {
     uint32_t *flush_buf = nullptr;
     size_t flush_words = 0;
     std::vector<void *> user_allocs;
+    std::vector<jl_kv8_workspace *> kv8_workspaces;
     jl_counters counters = {};
 };
 
@@ -185,6 +192,22 @@ int fail(jl_ctx *ctx, int code, const char *fmt, ...) {
     do {                                 \
         if (!(cond)) return fail(ctx, code, __VA_ARGS__); \
     } while (0)
+
+// The context's device as the current one for a call on a caller's stream; the caller's own device afterwards.
+struct DeviceGuard {
+    int before = -1, device;
+    explicit DeviceGuard(int d) : device(d) {
+        if (cudaGetDevice(&before) != cudaSuccess) before = -1;
+        if (before != device) cudaSetDevice(device);
+    }
+    ~DeviceGuard() {
+        if (before >= 0 && before != device) cudaSetDevice(before);
+    }
+};
+
+bool owns(const jl_ctx *ctx, const jl_kv8_workspace *ws) {
+    return std::find(ctx->kv8_workspaces.begin(), ctx->kv8_workspaces.end(), ws) != ctx->kv8_workspaces.end();
+}
 
 int dev_alloc(jl_ctx *ctx, void **p, size_t bytes) {
     cudaError_t e = cudaMalloc(p, bytes ? bytes : 16);
@@ -1265,6 +1288,10 @@ int32_t jl_destroy(jl_ctx *ctx) {
     if (ctx->nccl_comm) g_nccl.CommDestroy(ctx->nccl_comm);
     ctx->nccl_comm = nullptr;
     for (void *p : ctx->user_allocs) cudaFree(p);
+    for (jl_kv8_workspace *ws : ctx->kv8_workspaces) {
+        kv8_scratch_free(&ws->scratch);
+        delete ws;
+    }
     if (ctx->flush_buf) cudaFree(ctx->flush_buf);
     if (ctx->d_status) cudaFree(ctx->d_status);
     if (ctx->gemm_scratch) cudaFree(ctx->gemm_scratch);
@@ -2225,6 +2252,89 @@ int32_t jl_gemv(jl_ctx *ctx, int32_t ggml_type, int64_t rows, int64_t cols, cons
     }
     ctx->counters.h2d_bytes += size_t(n) * cols * 4;
     ctx->counters.d2h_bytes += size_t(n) * rows * 4;
+    return JL_OK;
+}
+
+// ---- 8-bit paged cache --------------------------------------------------------------------------
+
+int32_t jl_kv8_workspace_create(jl_ctx *ctx, jl_kv8_workspace **out) {
+    if (!ctx) return JL_ERR_INVALID;
+    JL_REQUIRE(ctx, out != nullptr, JL_ERR_INVALID, "out must not be NULL");
+    *out = nullptr;
+    DeviceGuard guard(ctx->device);
+    jl_kv8_workspace *ws = new (std::nothrow) jl_kv8_workspace();
+    JL_REQUIRE(ctx, ws != nullptr, JL_ERR_OOM, "host memory exhausted");
+    cudaError_t e = kv8_scratch_create(&ws->scratch, ctx->sm_count);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        kv8_scratch_free(&ws->scratch);
+        delete ws;
+        return fail(ctx, e == cudaErrorMemoryAllocation ? JL_ERR_OOM : JL_ERR_CUDA, "workspace allocation failed: %s", cudaGetErrorString(e));
+    }
+    ctx->kv8_workspaces.push_back(ws);
+    *out = ws;
+    return JL_OK;
+}
+
+int32_t jl_kv8_workspace_free(jl_ctx *ctx, jl_kv8_workspace *ws) {
+    if (!ctx || !ws) return JL_OK;
+    const auto at = std::find(ctx->kv8_workspaces.begin(), ctx->kv8_workspaces.end(), ws);
+    JL_REQUIRE(ctx, at != ctx->kv8_workspaces.end(), JL_ERR_INVALID, "this workspace is not one of the context's");
+    DeviceGuard guard(ctx->device);
+    kv8_scratch_free(&ws->scratch);  // cudaFree waits for what is under way
+    ctx->kv8_workspaces.erase(at);
+    delete ws;
+    return JL_OK;
+}
+
+int32_t jl_debug_kv8_check(int32_t which, const void *args, char *message, size_t n) {
+    if (!message || n == 0) return JL_ERR_INVALID;
+    message[0] = 0;
+    switch (which) {
+        case 0: return kv8_check_map(static_cast<const jl_kv8_map_args *>(args), message, n);
+        case 1: return kv8_check_append(static_cast<const jl_kv8_append_args *>(args), message, n);
+        case 2: return kv8_check_attention(static_cast<const jl_kv8_attention_args *>(args), message, n);
+        default: return JL_ERR_INVALID;
+    }
+}
+
+int32_t jl_kv8_map(jl_ctx *ctx, jl_kv8_workspace *ws, const jl_kv8_map_args *args, void *stream) {
+    if (!ctx) return JL_ERR_INVALID;
+    char message[512];
+    const int rc = kv8_check_map(args, message, sizeof message);
+    if (rc) return fail(ctx, rc, "%s", message);
+    JL_REQUIRE(ctx, owns(ctx, ws), JL_ERR_INVALID, "the workspace is not one of this context's");
+    DeviceGuard guard(ctx->device);
+    const cudaError_t e = kv8_map_launch(*args, ws->scratch, ctx->sm_count, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return fail(ctx, JL_ERR_CUDA, "block map launch failed: %s", cudaGetErrorString(e));
+    ctx->counters.kernel_launches++;
+    return JL_OK;
+}
+
+int32_t jl_kv8_append(jl_ctx *ctx, const jl_kv8_append_args *args, void *stream) {
+    if (!ctx) return JL_ERR_INVALID;
+    char message[512];
+    const int rc = kv8_check_append(args, message, sizeof message);
+    if (rc) return fail(ctx, rc, "%s", message);
+    if (args->tokens == 0) return JL_OK;
+    DeviceGuard guard(ctx->device);
+    const cudaError_t e = kv8_append_launch(*args, ctx->sm_count, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return fail(ctx, JL_ERR_CUDA, "append launch failed: %s", cudaGetErrorString(e));
+    ctx->counters.kernel_launches++;
+    return JL_OK;
+}
+
+int32_t jl_kv8_attention(jl_ctx *ctx, jl_kv8_workspace *ws, const jl_kv8_attention_args *args, void *stream) {
+    if (!ctx) return JL_ERR_INVALID;
+    char message[512];
+    const int rc = kv8_check_attention(args, message, sizeof message);
+    if (rc) return fail(ctx, rc, "%s", message);
+    JL_REQUIRE(ctx, owns(ctx, ws), JL_ERR_INVALID, "the workspace is not one of this context's");
+    if (args->rows == 0) return JL_OK;
+    DeviceGuard guard(ctx->device);
+    const cudaError_t e = kv8_attention_launch(*args, ws->scratch, ctx->sm_count, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return fail(ctx, JL_ERR_CUDA, "attention launch failed: %s", cudaGetErrorString(e));
+    ctx->counters.kernel_launches++;
     return JL_OK;
 }
 

@@ -1,0 +1,27 @@
+// The 8-bit paged key/value cache (jl_kv8_* of include/jitllm_b200.h): launches of kv8.cu and kv8_attention.cu.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include "../../include/jitllm_b200.h"
+
+namespace jl {
+
+// What is wrong with the arguments: a status and, unless it is JL_OK, a message of at most n - 1 characters.
+int kv8_check_map(const jl_kv8_map_args *a, char *message, size_t n);
+int kv8_check_append(const jl_kv8_append_args *a, char *message, size_t n);
+int kv8_check_attention(const jl_kv8_attention_args *a, char *message, size_t n);
+
+// The device half of a jl_kv8_workspace.
+struct Kv8Scratch {
+    void *memory = nullptr;
+};
+cudaError_t kv8_scratch_create(Kv8Scratch *s, int sm_count);
+void kv8_scratch_free(Kv8Scratch *s);
+
+// Arguments that have passed the checks, on the current device.
+cudaError_t kv8_map_launch(const jl_kv8_map_args &a, const Kv8Scratch &s, int sm_count, cudaStream_t stream);
+cudaError_t kv8_append_launch(const jl_kv8_append_args &a, int sm_count, cudaStream_t stream);
+cudaError_t kv8_attention_launch(const jl_kv8_attention_args &a, const Kv8Scratch &s, int sm_count, cudaStream_t stream);
+
+}  // namespace jl
