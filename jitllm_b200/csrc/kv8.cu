@@ -142,13 +142,6 @@ __global__ void __launch_bounds__(256) append_kernel(jl_kv8_append_args a) {
 
 }  // namespace
 
-cudaError_t kv8_scratch_create(Kv8Scratch *s, int) { return cudaMalloc(&s->memory, 256); }
-
-void kv8_scratch_free(Kv8Scratch *s) {
-    if (s->memory) cudaFree(s->memory);
-    s->memory = nullptr;
-}
-
 cudaError_t kv8_map_launch(const jl_kv8_map_args &a, const Kv8Scratch &, int, cudaStream_t stream) {
     map_kernel<<<1, kMapThreads, 0, stream>>>(a);
     return cudaGetLastError();

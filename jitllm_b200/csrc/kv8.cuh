@@ -12,7 +12,8 @@ int kv8_check_map(const jl_kv8_map_args *a, char *message, size_t n);
 int kv8_check_append(const jl_kv8_append_args *a, char *message, size_t n);
 int kv8_check_attention(const jl_kv8_attention_args *a, char *message, size_t n);
 
-// The device half of a jl_kv8_workspace.
+// The device half of a jl_kv8_workspace: counters that are zero between launches, then the attention's parts.
+constexpr size_t kKv8CounterBytes = 16384;
 struct Kv8Scratch {
     void *memory = nullptr;
 };

@@ -1,6 +1,21 @@
 // Attention of single tokens over the 8-bit paged key/value cache.
+//
+// Work. A unit is one row and up to eight query heads of one KV head; its tokens are cut into tiles of 64. The tiles of all units
+// form one line (rows in order, then heads, then tokens), of which every CTA of a grid that fits the GPU takes an equal piece. The
+// lengths are on the device, so each CTA works the line out for itself from the rows' positions. A unit that lies within a piece is
+// finished there; the parts of one that is cut are left in the workspace, and the CTA that arrives last at the unit's counter joins
+// them in order, so results do not hang on who arrives when.
+//
+// Mathematics. s = scale * ks_j * (q . kc_j), weights p_j = 2^(s_j log2 e - m) with a running maximum m, and
+// out = sum p_j vs_j vc_j / sum p_j. Codes are exact in binary16; a query is split into two binary16 parts of eleven bits each
+// (scaled by the power of two that takes its largest element to [2^14, 2^15)), and so is p_j vs_j. The parts of eight heads are
+// the sixteen rows of an mma.m16n8k16, so products are exact to 22 bits and sums are binary32. p_j vs_j has a running power of two E of its own
+// (w_j = 2^(s_j log2 e - E) vs_j, below 2^15): scales of values may differ by any factor between tokens. m and E are whole numbers, so that
+// moving them on rounds nothing.
 #include <cuda_fp16.h>
 #include <math_constants.h>
+
+#include <atomic>
 
 #include "common.cuh"
 #include "kv8.cuh"
@@ -9,106 +24,551 @@ namespace jl {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kMaxPairs = 4;  // pairs of elements that a lane has of a head of 256
+constexpr int kThreads = 32 * kWarps;
+constexpr int kStep = 16;                // tokens that a warp takes at a time
+constexpr int kTile = kStep * kWarps;    // tokens of a tile
+constexpr int kHeads = 8;                // query heads of a unit
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 
-// A CTA per row and query head: its warps take tokens in turn, one at a time, with a running maximum and sum (a rescaled
-// softmax, so one pass over the cache), and are folded at the end.
-__global__ void __launch_bounds__(32 * kWarps) attention_kernel(jl_kv8_attention_args a) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int r = blockIdx.x, h = blockIdx.y, d = a.pages.head_dim;
-    if (a.token_count && r >= a.token_count[0]) return;
-    const int kv = h / (a.heads / a.pages.kv_heads), bt = a.pages.block_tokens;
+// ---- layout of a stage in shared memory: 16 rows of keys, 16 rows of values, their scales, the mask of tokens that count -----------
+// Rows are read as 16-byte pieces across eight rows (keys) or every second row (values). With 64, 128 and 256 bytes a row, pieces are
+// exchanged within a 128-byte line so that both reads are free of bank conflicts; rows of 96 and 192 bytes are 16 bytes apart instead.
+template <int HD>
+struct Layout {
+    static constexpr int kPitch = HD == 96 || HD == 192 ? HD + 16 : HD;
+    static constexpr int kValues = kStep * kPitch, kScales = 2 * kValues, kMask = kScales + 2 * kStep * 4;
+    static constexpr int kStage = kMask + 16;
+    static constexpr int kStages = HD <= 128 ? 4 : 3;
+    static constexpr int kResident = HD <= 96 ? 4 : HD == 128 ? 3 : 2;  // CTAs per SM
+    static constexpr int kRing = kStages * kStage;
+    static constexpr int kOut = kHeads * HD;                            // floats of one part's outputs
+    static constexpr int kBytes = kWarps * (kRing > kOut * 4 ? kRing : kOut * 4);
+
+    // where 16-byte piece c of row r is
+    __device__ static int piece(int r, int c) {
+        if constexpr (HD == 64) return (r >> 1) * 128 + (((((r & 1) << 2) | c) ^ ((r >> 1 & 3) << 1)) << 4);
+        else if constexpr (HD == 128 || HD == 256) return r * HD + ((c ^ (r & 7)) << 4);
+        else return r * kPitch + (c << 4);
+    }
+    // byte (= element) of a row that lane t's word w of keys starts at
+    __device__ static int key_element(int t, int w) {
+        if constexpr (HD == 64) return t * 16 + w * 4;
+        else if constexpr (HD == 96) return (w >> 1) * 32 + t * 8 + (w & 1) * 4;
+        else if constexpr (HD == 192) return (w >> 2) * 64 + t * 16 + (w & 3) * 4;
+        else return (w >> 3) * 128 + t * 32 + (w & 7) * 4;
+    }
+    // byte of a row that lane g's word j of values starts at
+    __device__ static int value_element(int g, int j) {
+        if constexpr (HD == 64) return g * 8 + j * 4;
+        else if constexpr (HD == 96) return j * 32 + g * 4;
+        else if constexpr (HD == 192) return (j >> 1) * 64 + g * 8 + (j & 1) * 4;
+        else return (j >> 2) * 128 + g * 16 + (j & 3) * 4;
+    }
+};
+
+struct Params {
+    jl_kv8_attention_args a;
+    uint64_t divide;   // j / block_tokens = j * divide >> shift for j < 2^31
+    int shift;
+    int group, head_tiles, units;  // query heads per KV head, units per KV head and per row
+    unsigned *arrivals;            // [CTAs], zero between launches
+    float *parts;                  // [2 * CTAs][part floats]
+};
+template <int HD>
+constexpr int kPartFloats = Layout<HD>::kOut + 3 * kHeads;
+
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Two bytes (signed codes with their top bit flipped) as binary16: 0x64uu is 1024 + u, and u is code + 128.
+template <int SELECT>
+__device__ __forceinline__ uint32_t codes_to_half2(uint32_t flipped) {
+    const uint32_t biased = __byte_perm(flipped, 0x64646464u, SELECT);
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&biased), __half2half2(__ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t *>(&x);
+}
+__device__ __forceinline__ uint32_t pack(__half lo, __half hi) {
+    const __half2 x = __halves2half2(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&x);
+}
+// x and y as two binary16 parts each: `big` rounded to eleven bits, `rest` what that leaves.
+__device__ __forceinline__ void split(float x, float y, uint32_t &big, uint32_t &rest) {
+    const __half bx = __float2half_rn(x), by = __float2half_rn(y);
+    big = pack(bx, by);
+    rest = pack(__float2half_rn(x - __half2float(bx)), __float2half_rn(y - __half2float(by)));
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 2^(from - to) of whole numbers from <= to, exactly (from -inf: nothing is there, 0; below 2^-126: 0)
+__device__ __forceinline__ float step_down(float from, float to) {
+    const float magic = 12582912.f;  // 1.5 * 2^23: the sum's low bits are the whole number
+    return from == to ? 1.f : __int_as_float((__float_as_int(fmaxf(from - to, -127.f) + magic) - __float_as_int(magic) + 127) << 23);
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// A row's tokens [first, first + count) in its sequence's line of the table.
+struct Row {
+    uint32_t first, count;
+    int slot;
+};
+__device__ __forceinline__ Row row_at(const jl_kv8_attention_args &a, int r) {
     const int slot = a.kv_slots ? a.kv_slots[r] : r, pos = a.positions[r];
-    const bool there = slot >= 0 && slot < a.slots;
-    const int64_t length = there ? min(int64_t(pos) + 1, int64_t(a.blocks_per_slot) * bt) : 0;
-    const int64_t first = a.window > 0 ? max(int64_t(pos) + 1 - a.window, int64_t(0)) : 0;
-    const bool f16 = a.ggml_type == JL_F16, outside = a.rope_cos && pos >= a.rope_rows;
+    const int64_t end = int64_t(pos) + 1, length = min(end, int64_t(a.blocks_per_slot) * a.pages.block_tokens);
+    const int64_t first = a.window > 0 ? max(end - a.window, int64_t(0)) : 0;
+    Row row = {0, 0, slot};
+    if (slot >= 0 && slot < a.slots && first < length) row.first = uint32_t(first), row.count = uint32_t(length - first);
+    return row;
+}
+// Tiles of a row's unit: one at least, so that a row without tokens gets its zeros.
+__device__ __forceinline__ uint32_t tiles_of(const Row &row) { return max(1u, (row.count + kTile - 1) / kTile); }
 
-    float q[kMaxPairs][2], o[kMaxPairs][2];
+// Sum of v over the CTA's threads; `before`: over those in front of this one.
+__device__ __forceinline__ uint32_t block_sum(uint32_t v, uint32_t *before, uint32_t *warp_sums) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t s = v;
 #pragma unroll
-    for (int i = 0; i < kMaxPairs; ++i) {
-        const int e = 2 * (lane + 32 * i);
-        q[i][0] = q[i][1] = o[i][0] = o[i][1] = 0.f;
-        if (e >= d || pos < 0) continue;
-        const int64_t at = int64_t(r) * a.q_stride + int64_t(h) * d + e;
-        q[i][0] = f16 ? __half2float(static_cast<const __half *>(a.q)[at]) : static_cast<const float *>(a.q)[at];
-        q[i][1] = f16 ? __half2float(static_cast<const __half *>(a.q)[at + 1]) : static_cast<const float *>(a.q)[at + 1];
-        if (a.rope_cos) {
-            const int64_t angle = int64_t(outside ? 0 : pos) * (d / 2) + e / 2;
-            const float c = outside ? CUDART_NAN_F : a.rope_cos[angle], s = outside ? CUDART_NAN_F : a.rope_sin[angle];
-            const float rotated = q[i][0] * c - q[i][1] * s;
-            q[i][1] = q[i][0] * s + q[i][1] * c;
-            q[i][0] = rotated;
-        }
-    }
-    float most = -CUDART_INF_F, sum = 0.f;
-    for (int64_t j = first + warp; j < length; j += kWarps) {
-        const int block = a.block_table[int64_t(slot) * a.blocks_per_slot + j / bt];
-        if (block < 0 || block >= a.pages.blocks) continue;
-        const int64_t row = int64_t(kv) * bt + j % bt;
-        const int8_t *k = a.pages.k + block * a.pages.block_stride + row * d, *v = a.pages.v + block * a.pages.block_stride + row * d;
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < kMaxPairs; ++i) {
-            const int e = 2 * (lane + 32 * i);
-            if (e >= d) continue;
-            const char2 c = *reinterpret_cast<const char2 *>(k + e);
-            s += q[i][0] * float((signed char)c.x) + q[i][1] * float((signed char)c.y);
-        }
-#pragma unroll
-        for (int w = 16; w; w >>= 1) s += __shfl_xor_sync(~0u, s, w);
-        s *= a.scale * a.pages.k_scale[block * a.pages.scale_stride + row];
-        const float now = fmaxf(most, s), base = now == -CUDART_INF_F ? 0.f : now, keep = expf(most - base), p = expf(s - base);
-        // o is the mean of the values so far, which is never larger than they are; their sum could be beyond binary32
-        const float before = sum * keep, vs = a.pages.v_scale[block * a.pages.scale_stride + row];
-        most = now;
-        sum = before + p;
-        const float old = sum == 0.f ? 0.f : before / sum, fresh = sum == 0.f ? 0.f : p / sum;
-#pragma unroll
-        for (int i = 0; i < kMaxPairs; ++i) {
-            const int e = 2 * (lane + 32 * i);
-            if (e >= d) continue;
-            const char2 c = *reinterpret_cast<const char2 *>(v + e);
-            o[i][0] = o[i][0] * old + fresh * (vs * float((signed char)c.x));
-            o[i][1] = o[i][1] * old + fresh * (vs * float((signed char)c.y));
-        }
-    }
-    __shared__ float warp_most[kWarps], warp_sum[kWarps], warp_out[kWarps][64 * kMaxPairs];
-    if (lane == 0) {
-        warp_most[warp] = most;
-        warp_sum[warp] = sum;
-    }
-#pragma unroll
-    for (int i = 0; i < kMaxPairs; ++i) {
-        warp_out[warp][2 * (lane + 32 * i)] = o[i][0];
-        warp_out[warp][2 * (lane + 32 * i) + 1] = o[i][1];
+    for (int d = 1; d < 32; d <<= 1) {
+        const uint32_t o = __shfl_up_sync(~0u, s, d);
+        if (lane >= d) s += o;
     }
     __syncthreads();
-    float all = -CUDART_INF_F, total = 0.f;
-    for (int w = 0; w < kWarps; ++w) all = fmaxf(all, warp_most[w]);
-    const float base = all == -CUDART_INF_F ? 0.f : all;
-    float part[kWarps];
+    if (lane == 31) warp_sums[warp] = s;
+    __syncthreads();
+    uint32_t base = 0, all = 0;
+#pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-        part[w] = expf(warp_most[w] - base);
-        total += warp_sum[w] * part[w];
+        if (w < warp) base += warp_sums[w];
+        all += warp_sums[w];
     }
-    for (int e = threadIdx.x; e < d; e += 32 * kWarps) {
-        float x = 0.f;
-        for (int w = 0; w < kWarps; ++w) x += total == 0.f ? 0.f : warp_out[w][e] * (warp_sum[w] * part[w] / total);
-        const int64_t at = int64_t(r) * a.out_stride + int64_t(h) * d + e;
-        if (f16)
-            static_cast<__half *>(a.out)[at] = __float2half_rn(x);
-        else
-            static_cast<float *>(a.out)[at] = x;
-    }
-    if (a.lse && threadIdx.x == 0) a.lse[int64_t(r) * a.heads + h] = total == 0.f ? -CUDART_INF_F : base + logf(total);
+    *before = base + s - v;
+    return all;
 }
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads, Layout<HD>::kResident) attention_kernel(const Params p) {
+    using L = Layout<HD>;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ uint32_t warp_sums[kWarps], start_row, start_tile;
+    __shared__ float s_m[kWarps][kHeads], s_e[kWarps][kHeads], s_l[kWarps][kHeads];
+    __shared__ int last;
+    const jl_kv8_attention_args &a = p.a;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int rows = a.token_count ? min(a.token_count[0], a.rows) : a.rows;
+
+    // ---- this CTA's piece of the line of tiles
+    uint32_t total = 0;
+    for (int base = 0; base < rows; base += kThreads) {
+        const int r = base + tid;
+        total += r < rows ? tiles_of(row_at(a, r)) * p.units : 0;
+    }
+    uint32_t unused;
+    total = block_sum(total, &unused, warp_sums);
+    const uint32_t quota = (total + gridDim.x - 1) / gridDim.x;
+    uint32_t at = blockIdx.x * quota;
+    const uint32_t end = min(at + quota, total);
+    if (at >= end) return;
+    uint32_t front = 0;  // tiles in front of the rows from `base` on
+    for (int base = 0; base < rows; base += kThreads) {
+        const int r = base + tid;
+        const uint32_t mine = r < rows ? tiles_of(row_at(a, r)) * p.units : 0;
+        uint32_t before;
+        const uint32_t all = block_sum(mine, &before, warp_sums);
+        if (at >= front + before && at < front + before + mine) {
+            start_row = r;
+            start_tile = at - front - before;
+        }
+        front += all;
+        if (front > at) break;
+    }
+    __syncthreads();
+    int r = start_row;
+    uint32_t in_row = start_tile;
+
+    unsigned char *ring = smem + warp * L::kRing;
+    const uint32_t ring_at = smem_u32(ring);
+    const int bt = a.pages.block_tokens;
+    while (at < end) {
+        const Row row = row_at(a, r);
+        const uint32_t tiles = tiles_of(row);
+        const uint32_t unit = in_row / tiles, tile = in_row % tiles, take = min(tiles - tile, end - at);
+        const int kv = unit / p.head_tiles, head0 = (unit % p.head_tiles) * kHeads;  // head0: within the group
+        const uint32_t unit_start = at - tile;
+        // tokens of this piece, and the steps of them that this warp takes
+        const uint32_t from = row.first + tile * kTile, to = min(row.first + row.count, from + take * kTile);
+        const int steps = to > from ? int((to - from + kStep - 1) / kStep) : 0;
+        const int mine = steps > warp ? (steps - warp + kWarps - 1) / kWarps : 0;
+        const int32_t *line = a.block_table + int64_t(row.slot) * a.blocks_per_slot;
+
+        // Lanes i and i + 16 look up token i of a step.
+        auto token_of = [&](int i) { return from + uint32_t(warp + i * kWarps) * kStep + (lane & 15); };
+        auto block_of = [&](int i) {
+            const uint32_t j = token_of(i);
+            return i < mine && j < to ? line[uint32_t((j * p.divide) >> p.shift)] : -1;
+        };
+        auto issue = [&](int i, int block) {
+            if (i < mine) {
+                const uint32_t stage = ring_at + uint32_t(i % L::kStages) * L::kStage, j = token_of(i);
+                const bool good = j < to && block >= 0 && block < a.pages.blocks;
+                const int64_t in_block = int64_t(kv) * bt + (j - uint32_t((j * p.divide) >> p.shift) * bt);
+                const int64_t code_at = good ? block * a.pages.block_stride + in_block * HD : -1;
+                const unsigned mask = __ballot_sync(~0u, good);
+                if (lane == 0) *reinterpret_cast<unsigned *>(ring + (i % L::kStages) * L::kStage + L::kMask) = mask;
+                if (good) copy4(stage + L::kScales + 4 * lane, (lane < 16 ? a.pages.k_scale : a.pages.v_scale) + block * a.pages.scale_stride + in_block);
+#pragma unroll
+                for (int n = 0; n < HD / 32; ++n) {
+                    const int piece = n * 32 + lane, row16 = piece / (HD / 16), c = piece % (HD / 16);
+                    const int64_t src = __shfl_sync(~0u, code_at, row16);
+                    const uint32_t dst = stage + L::piece(row16, c);
+                    if (src >= 0) {
+                        copy16(dst, a.pages.k + src + c * 16);
+                        copy16(dst + L::kValues, a.pages.v + src + c * 16);
+                    }
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+#pragma unroll
+        for (int i = 0; i < L::kStages - 1; ++i) issue(i, block_of(i));
+        int next_block = block_of(L::kStages - 1);
+
+        // ---- queries of head g: rotated, scaled, split into two parts
+        uint32_t q_big[HD / 16][2], q_rest[HD / 16][2];
+        float factor;
+        const bool head_here = head0 + g < p.group;
+        if (mine > 0) {
+            float x[HD / 16][4], largest = 0.f;
+            bool finite = true;
+            const int pos = a.positions[r];
+            const bool outside = a.rope_cos && pos >= a.rope_rows;
+            const int64_t q_at = int64_t(r) * a.q_stride + int64_t(kv * p.group + head0 + g) * HD;
+#pragma unroll
+            for (int w = 0; w < HD / 16; ++w) {
+                const int e = L::key_element(t, w);
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (head_here) {
+                    if (a.ggml_type == JL_F16) {
+                        const uint2 h = *reinterpret_cast<const uint2 *>(static_cast<const __half *>(a.q) + q_at + e);
+                        const float2 lo = __half22float2(*reinterpret_cast<const __half2 *>(&h.x)), hi = __half22float2(*reinterpret_cast<const __half2 *>(&h.y));
+                        v = make_float4(lo.x, lo.y, hi.x, hi.y);
+                    } else {
+                        v = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + q_at + e);
+                    }
+                }
+                if (a.rope_cos && !outside) {
+                    const int64_t angle = int64_t(pos) * (HD / 2) + e / 2;
+                    const float2 c = *reinterpret_cast<const float2 *>(a.rope_cos + angle), s = *reinterpret_cast<const float2 *>(a.rope_sin + angle);
+                    v = make_float4(v.x * c.x - v.y * s.x, v.x * s.x + v.y * c.x, v.z * c.y - v.w * s.y, v.z * s.y + v.w * c.y);
+                }
+                x[w][0] = v.x, x[w][1] = v.y, x[w][2] = v.z, x[w][3] = v.w;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    finite = finite && isfinite(x[w][k]);
+                    largest = fmaxf(largest, fabsf(x[w][k]));
+                }
+            }
+            largest = fmaxf(largest, __shfl_xor_sync(~0u, largest, 1));
+            largest = fmaxf(largest, __shfl_xor_sync(~0u, largest, 2));
+            const unsigned all_finite = __ballot_sync(~0u, finite && !outside);
+            finite = (all_finite >> (lane & ~3) & 15) == 15;
+            // 2^(14 - exponent of the largest), at most 2^126
+            const int shift = finite && largest > 0.f ? min(14 - (int(__float_as_uint(largest) >> 23) - 127), 126) : 0;
+            const float up = __uint_as_float(uint32_t(127 + shift) << 23);
+            factor = finite ? a.scale * kLog2e * ldexpf(1.f, -shift) : CUDART_NAN_F;
+#pragma unroll
+            for (int w = 0; w < HD / 16; ++w)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    if (!finite) x[w][2 * k] = x[w][2 * k + 1] = 0.f;
+                    split(x[w][2 * k] * up, x[w][2 * k + 1] * up, q_big[w][k], q_rest[w][k]);
+                }
+        }
+
+        // ---- one pass over this warp's tokens
+        float m = -CUDART_INF_F, e = -CUDART_INF_F, l = 0.f, o[HD / 8][4];
+#pragma unroll
+        for (int n = 0; n < HD / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+        for (int i = 0; i < mine; ++i) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 2) : "memory");
+            __syncwarp();
+            issue(i + L::kStages - 1, next_block);
+            next_block = block_of(i + L::kStages);
+            const unsigned char *stage = ring + (i % L::kStages) * L::kStage;
+            const uint32_t stage_at = ring_at + (i % L::kStages) * L::kStage;
+
+            float s0[4] = {}, s1[4] = {};  // tokens 0-7 and 8-15: columns 2t, 2t + 1 of head g, big and rest
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                uint32_t kw[HD / 16];
+                const int rk = g + 8 * half;
+                if constexpr (HD == 96) {
+#pragma unroll
+                    for (int n = 0; n < 3; ++n) {
+                        const uint2 x = lds64(stage_at + rk * L::kPitch + L::key_element(t, 2 * n));
+                        kw[2 * n] = x.x, kw[2 * n + 1] = x.y;
+                    }
+                } else {
+#pragma unroll
+                    for (int n = 0; n < HD / 64; ++n) {
+                        const uint4 x = lds128(stage_at + L::piece(rk, L::key_element(t, 4 * n) >> 4));
+                        kw[4 * n] = x.x, kw[4 * n + 1] = x.y, kw[4 * n + 2] = x.z, kw[4 * n + 3] = x.w;
+                    }
+                }
+                float(&s)[4] = half ? s1 : s0;
+#pragma unroll
+                for (int w = 0; w < HD / 16; ++w) {
+                    const uint32_t u = kw[w] ^ 0x80808080u;
+                    mma(s, q_big[w][0], q_rest[w][0], q_big[w][1], q_rest[w][1], codes_to_half2<0x4140>(u), codes_to_half2<0x4342>(u));
+                }
+            }
+
+            // scores in units of ln 2, running maxima, weights
+            const unsigned mask = *reinterpret_cast<const unsigned *>(stage + L::kMask);
+            const float *ks = reinterpret_cast<const float *>(stage + L::kScales), *vs = ks + kStep;
+            float x[4], v[4], top = -CUDART_INF_F, etop = -CUDART_INF_F;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int j = 2 * t + (k & 1) + 8 * (k >> 1);
+                const bool counts = mask >> j & 1;
+                const float acc = k < 2 ? s0[k & 1] + s0[2 + (k & 1)] : s1[k & 1] + s1[2 + (k & 1)];
+                x[k] = counts ? acc * factor * ks[j] : -CUDART_INF_F;
+                v[k] = counts ? vs[j] : 0.f;
+                top = fmaxf(top, x[k]);
+                etop = fmaxf(etop, x[k] + fmaxf(float(int(__float_as_uint(v[k]) >> 23 & 255) - 127), -113.f));
+            }
+            top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+            etop = fmaxf(etop, __shfl_xor_sync(~0u, etop, 1));
+            top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+            etop = fmaxf(etop, __shfl_xor_sync(~0u, etop, 2));
+            const float m_new = fmaxf(m, ceilf(top)), e_new = fmaxf(e, ceilf(etop) - 14.f);
+            l *= step_down(m, m_new);
+            if (__any_sync(~0u, e != e_new)) {
+                const float keep = step_down(e, e_new);
+#pragma unroll
+                for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) o[n][k] *= keep;
+            }
+            m = m_new;
+            e = e_new;
+            const float m_base = m == -CUDART_INF_F ? 0.f : m, e_base = e == -CUDART_INF_F ? 0.f : e;
+            float w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                l += exp2_approx(x[k] - m_base);
+                w[k] = exp2_approx(x[k] - e_base) * v[k];
+            }
+            uint32_t big0, rest0, big1, rest1;
+            split(w[0], w[1], big0, rest0);
+            split(w[2], w[3], big1, rest1);
+
+            // values: tokens 2t, 2t + 1 and 2t + 8, 2t + 9, the elements of column g
+#pragma unroll
+            for (int n = 0; n < (HD >= 128 && HD != 192 ? HD / 128 : HD == 192 ? 3 : HD / 32 == 2 ? 1 : 3); ++n) {
+                constexpr int kWords = HD == 96 ? 1 : HD == 64 || HD == 192 ? 2 : 4;  // words of one load
+                uint32_t vw[4][kWords];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int rv = 2 * t + (k & 1) + 8 * (k >> 1);
+                    const int el = L::value_element(g, n * kWords);
+                    const uint32_t addr = stage_at + L::kValues + L::piece(rv, el >> 4) + (el & 15);
+                    if constexpr (kWords == 4) {
+                        const uint4 y = lds128(addr);
+                        vw[k][0] = y.x, vw[k][1] = y.y, vw[k][2] = y.z, vw[k][3] = y.w;
+                    } else if constexpr (kWords == 2) {
+                        const uint2 y = lds64(addr);
+                        vw[k][0] = y.x, vw[k][1] = y.y;
+                    } else {
+                        vw[k][0] = lds32(addr);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < kWords; ++j) {
+                    const uint32_t u0 = vw[0][j] ^ 0x80808080u, u1 = vw[1][j] ^ 0x80808080u, u2 = vw[2][j] ^ 0x80808080u, u3 = vw[3][j] ^ 0x80808080u;
+                    const uint32_t a01 = __byte_perm(u0, u1, 0x5140), a23 = __byte_perm(u0, u1, 0x7362);
+                    const uint32_t b01 = __byte_perm(u2, u3, 0x5140), b23 = __byte_perm(u2, u3, 0x7362);
+                    const int n0 = (n * kWords + j) * 4;
+                    mma(o[n0], big0, rest0, big1, rest1, codes_to_half2<0x4140>(a01), codes_to_half2<0x4140>(b01));
+                    mma(o[n0 + 1], big0, rest0, big1, rest1, codes_to_half2<0x4342>(a01), codes_to_half2<0x4342>(b01));
+                    mma(o[n0 + 2], big0, rest0, big1, rest1, codes_to_half2<0x4140>(a23), codes_to_half2<0x4140>(b23));
+                    mma(o[n0 + 3], big0, rest0, big1, rest1, codes_to_half2<0x4342>(a23), codes_to_half2<0x4342>(b23));
+                }
+            }
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        l += __shfl_xor_sync(~0u, l, 1);
+        l += __shfl_xor_sync(~0u, l, 2);
+
+        // ---- fold the warps. Outputs lie as [element of a column][head][column].
+        __syncthreads();  // the rings are free
+        float *out_w = reinterpret_cast<float *>(smem) + warp * L::kOut;
+        if (t == 0) s_m[warp][g] = m, s_e[warp][g] = e, s_l[warp][g] = l;
+#pragma unroll
+        for (int n = 0; n < HD / 8; ++n)
+            *reinterpret_cast<float2 *>(out_w + n * 64 + g * 8 + 2 * t) = make_float2(o[n][0] + o[n][2], o[n][1] + o[n][3]);
+        __syncthreads();
+        const int pair = tid & 63, head = pair >> 3, column = pair & 7;
+        float m_all = -CUDART_INF_F, e_all = -CUDART_INF_F, l_all = 0.f, keep[kWarps];
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) m_all = fmaxf(m_all, s_m[w][head]), e_all = fmaxf(e_all, s_e[w][head]);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            l_all += s_l[w][head] * step_down(s_m[w][head], m_all);
+            keep[w] = step_down(s_e[w][head], e_all);
+        }
+        const uint32_t first_cta = unit_start / quota, last_cta = (unit_start + tiles - 1) / quota;
+        const bool whole = first_cta == last_cta;
+        float *part = p.parts + (size_t(blockIdx.x) * 2 + (blockIdx.x == first_cta)) * kPartFloats<HD>;
+        // writes four elements of one column of a head
+        auto finish = [&](int quad, float4 x, float top, float etop, float sum) {
+            if (head0 + head >= p.group) return;
+            // 2^(etop - top) / sum, in two factors: either may be beyond binary32 where the output is not
+            const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+            const int power = sum == 0.f || etop == -CUDART_INF_F || top == -CUDART_INF_F ? 0 : int(etop - top);
+            const int h1 = power / 2;
+            const float f1 = inverse * ldexpf(1.f, h1), f2 = ldexpf(1.f, power - h1);
+            x = make_float4(x.x * f1 * f2, x.y * f1 * f2, x.z * f1 * f2, x.w * f1 * f2);
+            const int64_t out_at = int64_t(r) * a.out_stride + int64_t(kv * p.group + head0 + head) * HD + L::value_element(column, quad);
+            if (a.ggml_type == JL_F16) {
+                const uint2 h = make_uint2(pack(__float2half_rn(x.x), __float2half_rn(x.y)), pack(__float2half_rn(x.z), __float2half_rn(x.w)));
+                *reinterpret_cast<uint2 *>(static_cast<__half *>(a.out) + out_at) = h;
+            } else {
+                *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + out_at) = x;
+            }
+            if (a.lse && quad == 0 && column == 0)
+                a.lse[int64_t(r) * a.heads + kv * p.group + head0 + head] = sum == 0.f ? -CUDART_INF_F : top * kLn2 + logf(sum);
+        };
+#pragma unroll
+        for (int quad = tid >> 6; quad < HD / 32; quad += kThreads / 64) {
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float *src = reinterpret_cast<const float *>(smem) + w * L::kOut + quad * 256 + pair;
+                x.x += src[0] * keep[w], x.y += src[64] * keep[w], x.z += src[128] * keep[w], x.w += src[192] * keep[w];
+            }
+            if (whole) {
+                finish(quad, x, m_all, e_all, l_all);
+            } else {
+                float *dst = part + quad * 256 + pair;
+                dst[0] = x.x, dst[64] = x.y, dst[128] = x.z, dst[192] = x.w;
+            }
+        }
+        if (!whole) {
+            if (tid < 64 && column == 0) {
+                part[L::kOut + head] = m_all;
+                part[L::kOut + kHeads + head] = e_all;
+                part[L::kOut + 2 * kHeads + head] = l_all;
+            }
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) {
+                const unsigned others = last_cta - first_cta;
+                last = atomicInc(p.arrivals + first_cta, others) == others;  // the last one to come sets it back to zero
+                __threadfence();
+            }
+            __syncthreads();
+            if (last) {
+                const int n = int(last_cta - first_cta) + 1;
+                auto part_of = [&](int k) { return p.parts + (size_t(first_cta + k) * 2 + (k == 0)) * kPartFloats<HD>; };
+                float top = -CUDART_INF_F, etop = -CUDART_INF_F, sum = 0.f;
+                for (int k = 0; k < n; ++k) {
+                    top = fmaxf(top, __ldcg(part_of(k) + L::kOut + head));
+                    etop = fmaxf(etop, __ldcg(part_of(k) + L::kOut + kHeads + head));
+                }
+                for (int k = 0; k < n; ++k) sum += __ldcg(part_of(k) + L::kOut + 2 * kHeads + head) * step_down(__ldcg(part_of(k) + L::kOut + head), top);
+                for (int quad = tid >> 6; quad < HD / 32; quad += kThreads / 64) {
+                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int k = 0; k < n; ++k) {
+                        const float *src = part_of(k) + quad * 256 + pair;
+                        const float f = step_down(__ldcg(part_of(k) + L::kOut + kHeads + head), etop);
+                        x.x += __ldcg(src) * f, x.y += __ldcg(src + 64) * f, x.z += __ldcg(src + 128) * f, x.w += __ldcg(src + 192) * f;
+                    }
+                    finish(quad, x, top, etop, sum);
+                }
+            }
+        }
+        __syncthreads();  // shared memory is free for the next unit
+        at += take;
+        in_row += take;
+        if (in_row == tiles * uint32_t(p.units)) ++r, in_row = 0;
+    }
+}
+
+template <int HD>
+cudaError_t launch(Params &p, const Kv8Scratch &s, int sm_count, cudaStream_t stream) {
+    using L = Layout<HD>;
+    static std::atomic<uint64_t> configured{0};  // a bit for each device
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = uint64_t(1) << (device & 63);
+    if (device > 63 || !(configured.load(std::memory_order_acquire) & bit)) {
+        e = cudaFuncSetAttribute(attention_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
+        if (e != cudaSuccess) return e;
+        if (device <= 63) configured.fetch_or(bit, std::memory_order_release);
+    }
+    // never more CTAs than tiles if every row were as long as the table is
+    const jl_kv8_attention_args &a = p.a;
+    int64_t most = int64_t(a.blocks_per_slot) * a.pages.block_tokens;
+    if (a.window > 0) most = most < a.window ? most : a.window;
+    const int64_t tiles = (most + kTile - 1) / kTile * p.units * a.rows;
+    const int grid = int(tiles < int64_t(sm_count) * L::kResident ? tiles : int64_t(sm_count) * L::kResident);
+    p.arrivals = static_cast<unsigned *>(s.memory);
+    p.parts = reinterpret_cast<float *>(static_cast<char *>(s.memory) + kKv8CounterBytes);
+    attention_kernel<HD><<<grid, kThreads, L::kBytes, stream>>>(p);
+    return cudaGetLastError();
+}
+
+constexpr int kMostResident = 4;
+static_assert(Layout<64>::kResident <= kMostResident && Layout<128>::kResident <= kMostResident && Layout<256>::kResident <= kMostResident);
 
 }  // namespace
 
-cudaError_t kv8_attention_launch(const jl_kv8_attention_args &a, const Kv8Scratch &, int, cudaStream_t stream) {
-    attention_kernel<<<dim3(a.rows, a.heads), 32 * kWarps, 0, stream>>>(a);
-    return cudaGetLastError();
+cudaError_t kv8_scratch_create(Kv8Scratch *s, int sm_count) {
+    // two parts for each CTA of the largest grid, of the largest kind
+    size_t part = 0;
+    for (const size_t n : {Layout<64>::kResident * kPartFloats<64>, Layout<96>::kResident * kPartFloats<96>, Layout<128>::kResident * kPartFloats<128>,
+                           Layout<192>::kResident * kPartFloats<192>, Layout<256>::kResident * kPartFloats<256>})
+        part = part > n ? part : n;
+    if (size_t(sm_count) * kMostResident * 4 > kKv8CounterBytes) return cudaErrorInvalidValue;
+    cudaError_t e = cudaMalloc(&s->memory, kKv8CounterBytes + size_t(sm_count) * 2 * part * 4);
+    if (e == cudaSuccess) e = cudaMemset(s->memory, 0, kKv8CounterBytes);
+    if (e == cudaSuccess) e = cudaDeviceSynchronize();  // the memset is over before a launch on any stream
+    return e;
+}
+
+void kv8_scratch_free(Kv8Scratch *s) {
+    if (s->memory) cudaFree(s->memory);
+    s->memory = nullptr;
+}
+
+cudaError_t kv8_attention_launch(const jl_kv8_attention_args &a, const Kv8Scratch &s, int sm_count, cudaStream_t stream) {
+    Params p = {};
+    p.a = a;
+    int bits = 0;
+    while ((int64_t(1) << bits) < a.pages.block_tokens) ++bits;
+    // floor(2^(31 + bits) / n) + 1 gives exact quotients of 31-bit numbers by n <= 2^bits (Granlund and Montgomery 1994)
+    p.shift = 31 + bits;
+    p.divide = (uint64_t(1) << p.shift) / uint64_t(a.pages.block_tokens) + 1;
+    p.group = a.heads / a.pages.kv_heads;
+    p.head_tiles = (p.group + kHeads - 1) / kHeads;
+    p.units = p.head_tiles * a.pages.kv_heads;
+    switch (a.pages.head_dim) {
+        case 64: return launch<64>(p, s, sm_count, stream);
+        case 96: return launch<96>(p, s, sm_count, stream);
+        case 128: return launch<128>(p, s, sm_count, stream);
+        case 192: return launch<192>(p, s, sm_count, stream);
+        default: return launch<256>(p, s, sm_count, stream);
+    }
 }
 
 }  // namespace jl

@@ -97,6 +97,10 @@ int kv8_check_attention(const jl_kv8_attention_args *a, char *message, size_t n)
                 a->blocks_per_slot, a->window);
     KV8_REQUIRE(a->heads > 0 && a->heads % a->pages.kv_heads == 0 && a->heads <= 16384, JL_ERR_INVALID,
                 "heads must be a multiple of kv_heads and at most 16384, got %d and %d", a->heads, a->pages.kv_heads);
+    const int64_t tiles = (int64_t(a->blocks_per_slot) * a->pages.block_tokens + 63) / 64 * a->heads;
+    KV8_REQUIRE(a->rows == 0 || tiles <= INT32_MAX / a->rows, JL_ERR_UNSUPPORTED,
+                "rows times heads times the tokens of a table row must be below 2^37, got %d rows, %d heads, %d blocks of %d", a->rows, a->heads,
+                a->blocks_per_slot, a->pages.block_tokens);
     KV8_REQUIRE(std::isfinite(a->scale), JL_ERR_INVALID, "scale must be finite");
     const int64_t row = int64_t(a->heads) * a->pages.head_dim;
     if ((rc = check_rows("q", a->q, a->q_stride, row, a->ggml_type, message, n))) return rc;
