@@ -1,6 +1,6 @@
 // Attention of single tokens over the 8-bit paged key/value cache.
 //
-// Work. A unit is one row and up to eight query heads of one KV head; its tokens are cut into tiles of 64. The tiles of all units
+// Work. A unit is one row and four or eight query heads of one KV head; its tokens are cut into tiles of 64. The tiles of all units
 // form one line (rows in order, then heads, then tokens), of which every CTA of a grid that fits the GPU takes an equal piece. The
 // lengths are on the device, so each CTA works the line out for itself from the rows' positions. A unit that lies within a piece is
 // finished there; the parts of one that is cut are left in the workspace, and the CTA that arrives last at the unit's counter joins
@@ -8,9 +8,10 @@
 //
 // Mathematics. s = scale * ks_j * (q . kc_j), weights p_j = 2^(s_j log2 e - m) with a running maximum m, and
 // out = sum p_j vs_j vc_j / sum p_j. Codes are exact in binary16; a query is split into two binary16 parts of eleven bits each
-// (scaled by the power of two that takes its largest element to [2^14, 2^15)), and so is p_j vs_j. The parts of eight heads are
-// the sixteen rows of an mma.m16n8k16, so products are exact to 22 bits and sums are binary32. p_j vs_j has a running power of two E of its own
-// (w_j = 2^(s_j log2 e - E) vs_j, below 2^15): scales of values may differ by any factor between tokens. m and E are whole numbers, so that
+// (scaled by the power of two that takes its largest element to [2^14, 2^15)), and so is p_j vs_j. The two parts of four heads are
+// the eight columns of an mma.m16n8k16 whose sixteen rows are tokens (keys) or elements (values), so products are exact to 22 bits;
+// the instructions' sums of sixteen tokens are added in binary32. w_j = 2^(s_j log2 e - E) vs_j has a running power of two E of its
+// own that keeps it below 2^15: scales of values may differ by any factor between tokens. m and E are whole numbers, so that
 // moving them on rounds nothing.
 #include <cuda_fp16.h>
 #include <math_constants.h>
@@ -27,7 +28,6 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kStep = 16;                // tokens that a warp takes at a time
 constexpr int kTile = kStep * kWarps;    // tokens of a tile
-constexpr int kHeads = 8;                // query heads of a unit
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 
 // ---- layout of a stage in shared memory: 16 rows of keys, 16 rows of values, their scales, the mask of tokens that count -----------
@@ -38,11 +38,13 @@ struct Layout {
     static constexpr int kPitch = HD == 96 || HD == 192 ? HD + 16 : HD;
     static constexpr int kValues = kStep * kPitch, kScales = 2 * kValues, kMask = kScales + 2 * kStep * 4;
     static constexpr int kStage = kMask + 16;
-    static constexpr int kStages = HD <= 128 ? 4 : 3;
-    static constexpr int kResident = HD <= 96 ? 4 : HD == 128 ? 3 : 2;  // CTAs per SM
+    static constexpr int kStages = HD <= 96 ? 4 : 3;
+    static constexpr int kResident = HD <= 128 ? 4 : 2;  // CTAs per SM
     static constexpr int kRing = kStages * kStage;
-    static constexpr int kOut = kHeads * HD;                            // floats of one part's outputs
-    static constexpr int kBytes = kWarps * (kRing > kOut * 4 ? kRing : kOut * 4);
+    static constexpr int kQuads = HD / 32;               // groups of four elements that a lane has of a head's output
+    static constexpr int kLoad = HD == 96 ? 1 : HD == 64 || HD == 192 ? 2 : 4;  // quads that one load of values brings
+    static constexpr int kBytes = kWarps * kRing;        // also holds the warps' outputs: 8 heads of HD floats each
+    static_assert(kRing >= 8 * HD * 4);
 
     // where 16-byte piece c of row r is
     __device__ static int piece(int r, int c) {
@@ -74,8 +76,8 @@ struct Params {
     unsigned *arrivals;            // [CTAs], zero between launches
     float *parts;                  // [2 * CTAs][part floats]
 };
-template <int HD>
-constexpr int kPartFloats = Layout<HD>::kOut + 3 * kHeads;
+template <int HD, int NT>
+constexpr int kPartFloats = 4 * NT * (HD + 3);
 
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -116,21 +118,28 @@ __device__ __forceinline__ void copy4(uint32_t dst, const void *src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 
-// A row's tokens [first, first + count) in its sequence's line of the table.
+// The transpose of an 8 x 8 matrix of binary16 whose row g is held by lanes 4g .. 4g + 3, two columns each.
+__device__ __forceinline__ uint32_t transpose(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+// A row's tokens [first, end) in its sequence's line of the table.
 struct Row {
-    uint32_t first, count;
+    uint32_t first, end;
     int slot;
 };
 __device__ __forceinline__ Row row_at(const jl_kv8_attention_args &a, int r) {
     const int slot = a.kv_slots ? a.kv_slots[r] : r, pos = a.positions[r];
-    const int64_t end = int64_t(pos) + 1, length = min(end, int64_t(a.blocks_per_slot) * a.pages.block_tokens);
-    const int64_t first = a.window > 0 ? max(end - a.window, int64_t(0)) : 0;
+    const int64_t seen = int64_t(pos) + 1, length = min(seen, int64_t(a.blocks_per_slot) * a.pages.block_tokens);
+    const int64_t first = a.window > 0 ? max(seen - a.window, int64_t(0)) : 0;
     Row row = {0, 0, slot};
-    if (slot >= 0 && slot < a.slots && first < length) row.first = uint32_t(first), row.count = uint32_t(length - first);
+    if (slot >= 0 && slot < a.slots && first < length) row.first = uint32_t(first), row.end = uint32_t(length);
     return row;
 }
-// Tiles of a row's unit: one at least, so that a row without tokens gets its zeros.
-__device__ __forceinline__ uint32_t tiles_of(const Row &row) { return max(1u, (row.count + kTile - 1) / kTile); }
+// Tiles of a row's unit; the first begins at a multiple of 16 tokens. One at least, so that a row without tokens gets its zeros.
+__device__ __forceinline__ uint32_t tiles_of(const Row &row) { return max(1u, (row.end - (row.first & ~15u) + kTile - 1) / kTile); }
 
 // Sum of v over the CTA's threads; `before`: over those in front of this one.
 __device__ __forceinline__ uint32_t block_sum(uint32_t v, uint32_t *before, uint32_t *warp_sums) {
@@ -154,9 +163,11 @@ __device__ __forceinline__ uint32_t block_sum(uint32_t v, uint32_t *before, uint
     return all;
 }
 
-template <int HD>
+// NT: groups of four query heads. PAGED16: blocks are multiples of 16 tokens, so a step's sixteen rows lie behind one another.
+template <int HD, int NT, bool PAGED16>
 __global__ void __launch_bounds__(kThreads, Layout<HD>::kResident) attention_kernel(const Params p) {
     using L = Layout<HD>;
+    constexpr int kHeads = 4 * NT;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ uint32_t warp_sums[kWarps], start_row, start_tile;
     __shared__ float s_m[kWarps][kHeads], s_e[kWarps][kHeads], s_l[kWarps][kHeads];
@@ -165,23 +176,24 @@ __global__ void __launch_bounds__(kThreads, Layout<HD>::kResident) attention_ker
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int rows = a.token_count ? min(a.token_count[0], a.rows) : a.rows;
 
-    // ---- this CTA's piece of the line of tiles
+    // ---- this CTA's piece of the line of tiles: [total b / CTAs, total (b + 1) / CTAs), a tile at least for each CTA that has one
     uint32_t total = 0;
     for (int base = 0; base < rows; base += kThreads) {
         const int r = base + tid;
         total += r < rows ? tiles_of(row_at(a, r)) * p.units : 0;
     }
-    uint32_t unused;
-    total = block_sum(total, &unused, warp_sums);
-    const uint32_t quota = (total + gridDim.x - 1) / gridDim.x;
-    uint32_t at = blockIdx.x * quota;
-    const uint32_t end = min(at + quota, total);
-    if (at >= end) return;
+    uint32_t before;
+    total = block_sum(total, &before, warp_sums);
+    if (total == 0) return;
+    const uint32_t ctas = min(gridDim.x, total);
+    if (blockIdx.x >= ctas) return;
+    uint32_t at = uint32_t(uint64_t(total) * blockIdx.x / ctas);
+    const uint32_t end = uint32_t(uint64_t(total) * (blockIdx.x + 1) / ctas);
+    auto owner = [&](uint32_t tile) { return uint32_t(((uint64_t(tile) + 1) * ctas - 1) / total); };
     uint32_t front = 0;  // tiles in front of the rows from `base` on
     for (int base = 0; base < rows; base += kThreads) {
         const int r = base + tid;
         const uint32_t mine = r < rows ? tiles_of(row_at(a, r)) * p.units : 0;
-        uint32_t before;
         const uint32_t all = block_sum(mine, &before, warp_sums);
         if (at >= front + before && at < front + before + mine) {
             start_row = r;
@@ -203,188 +215,235 @@ __global__ void __launch_bounds__(kThreads, Layout<HD>::kResident) attention_ker
         const uint32_t unit = in_row / tiles, tile = in_row % tiles, take = min(tiles - tile, end - at);
         const int kv = unit / p.head_tiles, head0 = (unit % p.head_tiles) * kHeads;  // head0: within the group
         const uint32_t unit_start = at - tile;
-        // tokens of this piece, and the steps of them that this warp takes
-        const uint32_t from = row.first + tile * kTile, to = min(row.first + row.count, from + take * kTile);
+        // tokens of this piece, and the steps of them that this warp takes: i from 0 on, at token from + (warp + 4 i) 16
+        const uint32_t from = (row.first & ~15u) + tile * kTile, to = min(row.end, from + take * kTile);
         const int steps = to > from ? int((to - from + kStep - 1) / kStep) : 0;
         const int mine = steps > warp ? (steps - warp + kWarps - 1) / kWarps : 0;
         const int32_t *line = a.block_table + int64_t(row.slot) * a.blocks_per_slot;
+        auto step_at = [&](int i) { return from + uint32_t(warp + i * kWarps) * kStep; };
+        auto block_of = [&](uint32_t j) { return uint32_t((j * p.divide) >> p.shift); };
 
-        // Lanes i and i + 16 look up token i of a step.
-        auto token_of = [&](int i) { return from + uint32_t(warp + i * kWarps) * kStep + (lane & 15); };
-        auto block_of = [&](int i) {
-            const uint32_t j = token_of(i);
-            return i < mine && j < to ? line[uint32_t((j * p.divide) >> p.shift)] : -1;
+        // PAGED16: lane i looks up step 32 k + i of this warp, 32 steps ahead; where its codes and scales begin, or -1.
+        // Otherwise lanes i and i + 16 look up token i of a step, one step ahead.
+        int64_t code_at = -1, scale_at = -1;
+        int ahead;
+        auto look_up = [&](int i) {
+            if constexpr (PAGED16) return i + lane < mine ? line[block_of(step_at(i + lane))] : -1;
+            const uint32_t j = step_at(i) + (lane & 15);
+            return i < mine && j < to ? line[block_of(j)] : -1;
         };
-        auto issue = [&](int i, int block) {
+        auto place = [&](int block, uint32_t j) {
+            const bool good = block >= 0 && block < a.pages.blocks;
+            const int64_t in_block = int64_t(kv) * bt + (j - block_of(j) * bt);
+            code_at = good ? block * a.pages.block_stride + in_block * HD : -1;
+            scale_at = block * a.pages.scale_stride + in_block;
+        };
+        auto issue = [&](int i) {
             if (i < mine) {
-                const uint32_t stage = ring_at + uint32_t(i % L::kStages) * L::kStage, j = token_of(i);
-                const bool good = j < to && block >= 0 && block < a.pages.blocks;
-                const int64_t in_block = int64_t(kv) * bt + (j - uint32_t((j * p.divide) >> p.shift) * bt);
-                const int64_t code_at = good ? block * a.pages.block_stride + in_block * HD : -1;
-                const unsigned mask = __ballot_sync(~0u, good);
-                if (lane == 0) *reinterpret_cast<unsigned *>(ring + (i % L::kStages) * L::kStage + L::kMask) = mask;
-                if (good) copy4(stage + L::kScales + 4 * lane, (lane < 16 ? a.pages.k_scale : a.pages.v_scale) + block * a.pages.scale_stride + in_block);
+                const uint32_t stage = ring_at + uint32_t(i % L::kStages) * L::kStage, j0 = step_at(i);
+                unsigned mask = (j0 < row.first ? 0xffffu << (row.first - j0) : 0xffffu) & (to - j0 < 16 ? (1u << (to - j0)) - 1 : 0xffffu);
+                if constexpr (PAGED16) {
+                    if (i % 32 == 0) {
+                        place(ahead, step_at(i + lane));
+                        ahead = look_up(i + 32);
+                    }
+                    const int64_t code = __shfl_sync(~0u, code_at, i & 31), scale = __shfl_sync(~0u, scale_at, i & 31);
+                    if (code < 0) mask = 0;
+                    if (code >= 0) {
+                        const int8_t *k = a.pages.k + code + lane * 16, *v = a.pages.v + code + lane * 16;
+                        copy4(stage + L::kScales + 4 * lane, (lane < 16 ? a.pages.k_scale : a.pages.v_scale) + scale + (lane & 15));
 #pragma unroll
-                for (int n = 0; n < HD / 32; ++n) {
-                    const int piece = n * 32 + lane, row16 = piece / (HD / 16), c = piece % (HD / 16);
-                    const int64_t src = __shfl_sync(~0u, code_at, row16);
-                    const uint32_t dst = stage + L::piece(row16, c);
-                    if (src >= 0) {
-                        copy16(dst, a.pages.k + src + c * 16);
-                        copy16(dst + L::kValues, a.pages.v + src + c * 16);
+                        for (int n = 0; n < HD / 32; ++n) {
+                            const int piece = n * 32 + lane;
+                            const uint32_t dst = stage + L::piece(piece / (HD / 16), piece % (HD / 16));
+                            copy16(dst, k + n * 512);
+                            copy16(dst + L::kValues, v + n * 512);
+                        }
+                    }
+                } else {
+                    place(ahead, j0 + (lane & 15));
+                    ahead = look_up(i + 1);
+                    mask &= __ballot_sync(~0u, code_at >= 0);
+                    if (code_at >= 0) copy4(stage + L::kScales + 4 * lane, (lane < 16 ? a.pages.k_scale : a.pages.v_scale) + scale_at);
+#pragma unroll
+                    for (int n = 0; n < HD / 32; ++n) {
+                        const int piece = n * 32 + lane, row16 = piece / (HD / 16), c = piece % (HD / 16);
+                        const int64_t src = __shfl_sync(~0u, code_at, row16);
+                        const uint32_t dst = stage + L::piece(row16, c);
+                        if (src >= 0) {
+                            copy16(dst, a.pages.k + src + c * 16);
+                            copy16(dst + L::kValues, a.pages.v + src + c * 16);
+                        }
                     }
                 }
+                if (lane == 0) *reinterpret_cast<unsigned *>(ring + (i % L::kStages) * L::kStage + L::kMask) = mask;
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
+        ahead = look_up(0);
 #pragma unroll
-        for (int i = 0; i < L::kStages - 1; ++i) issue(i, block_of(i));
-        int next_block = block_of(L::kStages - 1);
+        for (int i = 0; i < L::kStages - 1; ++i) issue(i);
 
-        // ---- queries of head g: rotated, scaled, split into two parts
-        uint32_t q_big[HD / 16][2], q_rest[HD / 16][2];
-        float factor;
-        const bool head_here = head0 + g < p.group;
+        // ---- queries: column g of group n is part g & 1 of head 4 n + g / 2. Rotated, scaled, split.
+        uint32_t q[NT][HD / 16][2];
+        float factor[NT];  // of head 4 n + t
         if (mine > 0) {
-            float x[HD / 16][4], largest = 0.f;
-            bool finite = true;
             const int pos = a.positions[r];
             const bool outside = a.rope_cos && pos >= a.rope_rows;
-            const int64_t q_at = int64_t(r) * a.q_stride + int64_t(kv * p.group + head0 + g) * HD;
 #pragma unroll
-            for (int w = 0; w < HD / 16; ++w) {
-                const int e = L::key_element(t, w);
-                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (head_here) {
-                    if (a.ggml_type == JL_F16) {
-                        const uint2 h = *reinterpret_cast<const uint2 *>(static_cast<const __half *>(a.q) + q_at + e);
-                        const float2 lo = __half22float2(*reinterpret_cast<const __half2 *>(&h.x)), hi = __half22float2(*reinterpret_cast<const __half2 *>(&h.y));
-                        v = make_float4(lo.x, lo.y, hi.x, hi.y);
-                    } else {
-                        v = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + q_at + e);
+            for (int n = 0; n < NT; ++n) {
+                const int head = head0 + 4 * n + (g >> 1);
+                float x[HD / 16][4], largest = 0.f;
+                bool finite = !outside;
+                const int64_t q_at = int64_t(r) * a.q_stride + int64_t(kv * p.group + head) * HD;
+#pragma unroll
+                for (int w = 0; w < HD / 16; ++w) {
+                    const int e = L::key_element(t, w);
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (head < p.group) {
+                        if (a.ggml_type == JL_F16) {
+                            const uint2 h = *reinterpret_cast<const uint2 *>(static_cast<const __half *>(a.q) + q_at + e);
+                            const float2 lo = __half22float2(*reinterpret_cast<const __half2 *>(&h.x)), hi = __half22float2(*reinterpret_cast<const __half2 *>(&h.y));
+                            v = make_float4(lo.x, lo.y, hi.x, hi.y);
+                        } else {
+                            v = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + q_at + e);
+                        }
+                    }
+                    if (a.rope_cos && !outside) {
+                        const int64_t angle = int64_t(pos) * (HD / 2) + e / 2;
+                        const float2 c = *reinterpret_cast<const float2 *>(a.rope_cos + angle), s = *reinterpret_cast<const float2 *>(a.rope_sin + angle);
+                        v = make_float4(v.x * c.x - v.y * s.x, v.x * s.x + v.y * c.x, v.z * c.y - v.w * s.y, v.z * s.y + v.w * c.y);
+                    }
+                    x[w][0] = v.x, x[w][1] = v.y, x[w][2] = v.z, x[w][3] = v.w;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        finite = finite && isfinite(x[w][k]);
+                        largest = fmaxf(largest, fabsf(x[w][k]));
                     }
                 }
-                if (a.rope_cos && !outside) {
-                    const int64_t angle = int64_t(pos) * (HD / 2) + e / 2;
-                    const float2 c = *reinterpret_cast<const float2 *>(a.rope_cos + angle), s = *reinterpret_cast<const float2 *>(a.rope_sin + angle);
-                    v = make_float4(v.x * c.x - v.y * s.x, v.x * s.x + v.y * c.x, v.z * c.y - v.w * s.y, v.z * s.y + v.w * c.y);
-                }
-                x[w][0] = v.x, x[w][1] = v.y, x[w][2] = v.z, x[w][3] = v.w;
+                largest = fmaxf(largest, __shfl_xor_sync(~0u, largest, 1));
+                largest = fmaxf(largest, __shfl_xor_sync(~0u, largest, 2));
+                finite = (__ballot_sync(~0u, finite) >> (lane & ~3) & 15) == 15;
+                // 2^(14 - exponent of the largest), at most 2^126
+                const int shift = finite && largest > 0.f ? min(14 - (int(__float_as_uint(largest) >> 23) - 127), 126) : 0;
+                const float up = __uint_as_float(uint32_t(127 + shift) << 23);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    finite = finite && isfinite(x[w][k]);
-                    largest = fmaxf(largest, fabsf(x[w][k]));
-                }
+                for (int w = 0; w < HD / 16; ++w)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        uint32_t big, rest;
+                        split(finite ? x[w][2 * k] * up : 0.f, finite ? x[w][2 * k + 1] * up : 0.f, big, rest);
+                        q[n][w][k] = g & 1 ? rest : big;
+                    }
+                // head 4 n + t is that of lanes with g = 2 t
+                factor[n] = __shfl_sync(~0u, finite ? a.scale * kLog2e * ldexpf(1.f, -shift) : CUDART_NAN_F, t * 8);
             }
-            largest = fmaxf(largest, __shfl_xor_sync(~0u, largest, 1));
-            largest = fmaxf(largest, __shfl_xor_sync(~0u, largest, 2));
-            const unsigned all_finite = __ballot_sync(~0u, finite && !outside);
-            finite = (all_finite >> (lane & ~3) & 15) == 15;
-            // 2^(14 - exponent of the largest), at most 2^126
-            const int shift = finite && largest > 0.f ? min(14 - (int(__float_as_uint(largest) >> 23) - 127), 126) : 0;
-            const float up = __uint_as_float(uint32_t(127 + shift) << 23);
-            factor = finite ? a.scale * kLog2e * ldexpf(1.f, -shift) : CUDART_NAN_F;
-#pragma unroll
-            for (int w = 0; w < HD / 16; ++w)
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    if (!finite) x[w][2 * k] = x[w][2 * k + 1] = 0.f;
-                    split(x[w][2 * k] * up, x[w][2 * k + 1] * up, q_big[w][k], q_rest[w][k]);
-                }
         }
 
-        // ---- one pass over this warp's tokens
-        float m = -CUDART_INF_F, e = -CUDART_INF_F, l = 0.f, o[HD / 8][4];
+        // ---- one pass over this warp's tokens: lane (g, t) has tokens g and g + 8 of a step, heads 4 n + t, elements of column g
+        float m[NT], e[NT], l[NT], o[NT][L::kQuads][4];
 #pragma unroll
-        for (int n = 0; n < HD / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+        for (int n = 0; n < NT; ++n) {
+            m[n] = e[n] = -CUDART_INF_F;
+            l[n] = 0.f;
+#pragma unroll
+            for (int j = 0; j < L::kQuads; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
+        }
         for (int i = 0; i < mine; ++i) {
             asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 2) : "memory");
             __syncwarp();
-            issue(i + L::kStages - 1, next_block);
-            next_block = block_of(i + L::kStages);
+            issue(i + L::kStages - 1);
             const unsigned char *stage = ring + (i % L::kStages) * L::kStage;
             const uint32_t stage_at = ring_at + (i % L::kStages) * L::kStage;
 
-            float s0[4] = {}, s1[4] = {};  // tokens 0-7 and 8-15: columns 2t, 2t + 1 of head g, big and rest
+            float s[NT][4] = {};
+            {
+                uint32_t kw[2][HD / 16];  // tokens g and g + 8
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                uint32_t kw[HD / 16];
-                const int rk = g + 8 * half;
-                if constexpr (HD == 96) {
+                for (int half = 0; half < 2; ++half) {
+                    const int rk = g + 8 * half;
+                    if constexpr (HD == 96) {
 #pragma unroll
-                    for (int n = 0; n < 3; ++n) {
-                        const uint2 x = lds64(stage_at + rk * L::kPitch + L::key_element(t, 2 * n));
-                        kw[2 * n] = x.x, kw[2 * n + 1] = x.y;
-                    }
-                } else {
+                        for (int w = 0; w < HD / 16; w += 2) {
+                            const uint2 x = lds64(stage_at + rk * L::kPitch + L::key_element(t, w));
+                            kw[half][w] = x.x, kw[half][w + 1] = x.y;
+                        }
+                    } else {
 #pragma unroll
-                    for (int n = 0; n < HD / 64; ++n) {
-                        const uint4 x = lds128(stage_at + L::piece(rk, L::key_element(t, 4 * n) >> 4));
-                        kw[4 * n] = x.x, kw[4 * n + 1] = x.y, kw[4 * n + 2] = x.z, kw[4 * n + 3] = x.w;
+                        for (int w = 0; w < HD / 16; w += 4) {
+                            const uint4 x = lds128(stage_at + L::piece(rk, L::key_element(t, w) >> 4));
+                            kw[half][w] = x.x, kw[half][w + 1] = x.y, kw[half][w + 2] = x.z, kw[half][w + 3] = x.w;
+                        }
                     }
                 }
-                float(&s)[4] = half ? s1 : s0;
 #pragma unroll
                 for (int w = 0; w < HD / 16; ++w) {
-                    const uint32_t u = kw[w] ^ 0x80808080u;
-                    mma(s, q_big[w][0], q_rest[w][0], q_big[w][1], q_rest[w][1], codes_to_half2<0x4140>(u), codes_to_half2<0x4342>(u));
+                    const uint32_t u0 = kw[0][w] ^ 0x80808080u, u1 = kw[1][w] ^ 0x80808080u;
+                    const uint32_t a0 = codes_to_half2<0x4140>(u0), a1 = codes_to_half2<0x4140>(u1), a2 = codes_to_half2<0x4342>(u0), a3 = codes_to_half2<0x4342>(u1);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) mma(s[n], a0, a1, a2, a3, q[n][w][0], q[n][w][1]);
                 }
             }
 
-            // scores in units of ln 2, running maxima, weights
+            // scores in units of ln 2 and weights; maxima are moved on where a score or a weight is beyond them
             const unsigned mask = *reinterpret_cast<const unsigned *>(stage + L::kMask);
             const float *ks = reinterpret_cast<const float *>(stage + L::kScales), *vs = ks + kStep;
-            float x[4], v[4], top = -CUDART_INF_F, etop = -CUDART_INF_F;
+            const bool counts[2] = {bool(mask >> g & 1), bool(mask >> (g + 8) & 1)};
+            const float key_scale[2] = {ks[g], ks[g + 8]}, v[2] = {counts[0] ? vs[g] : 0.f, counts[1] ? vs[g + 8] : 0.f};
+            uint32_t b[NT][2];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int j = 2 * t + (k & 1) + 8 * (k >> 1);
-                const bool counts = mask >> j & 1;
-                const float acc = k < 2 ? s0[k & 1] + s0[2 + (k & 1)] : s1[k & 1] + s1[2 + (k & 1)];
-                x[k] = counts ? acc * factor * ks[j] : -CUDART_INF_F;
-                v[k] = counts ? vs[j] : 0.f;
-                top = fmaxf(top, x[k]);
-                etop = fmaxf(etop, x[k] + fmaxf(float(int(__float_as_uint(v[k]) >> 23 & 255) - 127), -113.f));
+            for (int n = 0; n < NT; ++n) {
+                float x[2], w[2];
+                bool beyond = false;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    x[k] = counts[k] ? (s[n][2 * k] + s[n][2 * k + 1]) * factor[n] * key_scale[k] : -CUDART_INF_F;
+                    w[k] = exp2_approx(x[k] - e[n]) * v[k];
+                    beyond = beyond || x[k] > m[n] || fabsf(w[k]) > 32768.f;
+                }
+                if (__any_sync(~0u, beyond)) {
+                    float top = fmaxf(x[0], x[1]), etop = -CUDART_INF_F;
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) etop = fmaxf(etop, x[k] + fmaxf(float(int(__float_as_uint(v[k]) >> 23 & 255) - 127), -113.f));
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) {
+                        top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+                        etop = fmaxf(etop, __shfl_xor_sync(~0u, etop, d));
+                    }
+                    const float m_new = fmaxf(m[n], ceilf(top)), e_new = fmaxf(e[n], ceilf(etop) - 14.f), keep = step_down(e[n], e_new);
+                    l[n] *= step_down(m[n], m_new);
+#pragma unroll
+                    for (int j = 0; j < L::kQuads; ++j)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) o[n][j][k] *= keep;
+                    m[n] = m_new;
+                    e[n] = e_new;
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) w[k] = exp2_approx(x[k] - e[n]) * v[k];
+                }
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    // nothing has been seen yet (m = E = -inf, which -inf may not be taken from), or a token does not count
+                    const bool none = x[k] == -CUDART_INF_F;
+                    l[n] += none ? 0.f : exp2_approx(x[k] - m[n]);
+                    const float y = none ? 0.f * v[k] : w[k];
+                    const __half big = __float2half_rn(y);
+                    b[n][k] = transpose(pack(big, __float2half_rn(y - __half2float(big))));
+                }
             }
-            top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-            etop = fmaxf(etop, __shfl_xor_sync(~0u, etop, 1));
-            top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-            etop = fmaxf(etop, __shfl_xor_sync(~0u, etop, 2));
-            const float m_new = fmaxf(m, ceilf(top)), e_new = fmaxf(e, ceilf(etop) - 14.f);
-            l *= step_down(m, m_new);
-            if (__any_sync(~0u, e != e_new)) {
-                const float keep = step_down(e, e_new);
-#pragma unroll
-                for (int n = 0; n < HD / 8; ++n)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) o[n][k] *= keep;
-            }
-            m = m_new;
-            e = e_new;
-            const float m_base = m == -CUDART_INF_F ? 0.f : m, e_base = e == -CUDART_INF_F ? 0.f : e;
-            float w[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                l += exp2_approx(x[k] - m_base);
-                w[k] = exp2_approx(x[k] - e_base) * v[k];
-            }
-            uint32_t big0, rest0, big1, rest1;
-            split(w[0], w[1], big0, rest0);
-            split(w[2], w[3], big1, rest1);
 
-            // values: tokens 2t, 2t + 1 and 2t + 8, 2t + 9, the elements of column g
+            // values: of word j of column g, elements 0 and 1 are rows g and g + 8 of one product, 2 and 3 of the next
 #pragma unroll
-            for (int n = 0; n < (HD >= 128 && HD != 192 ? HD / 128 : HD == 192 ? 3 : HD / 32 == 2 ? 1 : 3); ++n) {
-                constexpr int kWords = HD == 96 ? 1 : HD == 64 || HD == 192 ? 2 : 4;  // words of one load
-                uint32_t vw[4][kWords];
+            for (int j0 = 0; j0 < L::kQuads; j0 += L::kLoad) {
+                uint32_t vw[4][L::kLoad];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const int rv = 2 * t + (k & 1) + 8 * (k >> 1);
-                    const int el = L::value_element(g, n * kWords);
+                    const int rv = 2 * t + (k & 1) + 8 * (k >> 1), el = L::value_element(g, j0);
                     const uint32_t addr = stage_at + L::kValues + L::piece(rv, el >> 4) + (el & 15);
-                    if constexpr (kWords == 4) {
+                    if constexpr (L::kLoad == 4) {
                         const uint4 y = lds128(addr);
                         vw[k][0] = y.x, vw[k][1] = y.y, vw[k][2] = y.z, vw[k][3] = y.w;
-                    } else if constexpr (kWords == 2) {
+                    } else if constexpr (L::kLoad == 2) {
                         const uint2 y = lds64(addr);
                         vw[k][0] = y.x, vw[k][1] = y.y;
                     } else {
@@ -392,44 +451,43 @@ __global__ void __launch_bounds__(kThreads, Layout<HD>::kResident) attention_ker
                     }
                 }
 #pragma unroll
-                for (int j = 0; j < kWords; ++j) {
+                for (int j = 0; j < L::kLoad; ++j) {
                     const uint32_t u0 = vw[0][j] ^ 0x80808080u, u1 = vw[1][j] ^ 0x80808080u, u2 = vw[2][j] ^ 0x80808080u, u3 = vw[3][j] ^ 0x80808080u;
-                    const uint32_t a01 = __byte_perm(u0, u1, 0x5140), a23 = __byte_perm(u0, u1, 0x7362);
-                    const uint32_t b01 = __byte_perm(u2, u3, 0x5140), b23 = __byte_perm(u2, u3, 0x7362);
-                    const int n0 = (n * kWords + j) * 4;
-                    mma(o[n0], big0, rest0, big1, rest1, codes_to_half2<0x4140>(a01), codes_to_half2<0x4140>(b01));
-                    mma(o[n0 + 1], big0, rest0, big1, rest1, codes_to_half2<0x4342>(a01), codes_to_half2<0x4342>(b01));
-                    mma(o[n0 + 2], big0, rest0, big1, rest1, codes_to_half2<0x4140>(a23), codes_to_half2<0x4140>(b23));
-                    mma(o[n0 + 3], big0, rest0, big1, rest1, codes_to_half2<0x4342>(a23), codes_to_half2<0x4342>(b23));
+                    const uint32_t near01 = __byte_perm(u0, u1, 0x5140), near23 = __byte_perm(u0, u1, 0x7362);
+                    const uint32_t far01 = __byte_perm(u2, u3, 0x5140), far23 = __byte_perm(u2, u3, 0x7362);
+                    const uint32_t x0 = codes_to_half2<0x4140>(near01), x1 = codes_to_half2<0x4342>(near01), x2 = codes_to_half2<0x4140>(far01), x3 = codes_to_half2<0x4342>(far01);
+                    const uint32_t y0 = codes_to_half2<0x4140>(near23), y1 = codes_to_half2<0x4342>(near23), y2 = codes_to_half2<0x4140>(far23), y3 = codes_to_half2<0x4342>(far23);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        float c[4] = {}, d[4] = {};
+                        mma(c, x0, x1, x2, x3, b[n][0], b[n][1]);
+                        mma(d, y0, y1, y2, y3, b[n][0], b[n][1]);
+                        float(&out)[4] = o[n][j0 + j];
+                        out[0] += c[0] + c[1], out[1] += c[2] + c[3], out[2] += d[0] + d[1], out[3] += d[2] + d[3];
+                    }
                 }
             }
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
-        l += __shfl_xor_sync(~0u, l, 1);
-        l += __shfl_xor_sync(~0u, l, 2);
 
-        // ---- fold the warps. Outputs lie as [element of a column][head][column].
+        // ---- fold the warps. Outputs lie as [group][quad][lane], four elements of head t each.
         __syncthreads();  // the rings are free
-        float *out_w = reinterpret_cast<float *>(smem) + warp * L::kOut;
-        if (t == 0) s_m[warp][g] = m, s_e[warp][g] = e, s_l[warp][g] = l;
+        float4 *out_w = reinterpret_cast<float4 *>(smem) + warp * NT * L::kQuads * 32;
 #pragma unroll
-        for (int n = 0; n < HD / 8; ++n)
-            *reinterpret_cast<float2 *>(out_w + n * 64 + g * 8 + 2 * t) = make_float2(o[n][0] + o[n][2], o[n][1] + o[n][3]);
-        __syncthreads();
-        const int pair = tid & 63, head = pair >> 3, column = pair & 7;
-        float m_all = -CUDART_INF_F, e_all = -CUDART_INF_F, l_all = 0.f, keep[kWarps];
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) m_all = fmaxf(m_all, s_m[w][head]), e_all = fmaxf(e_all, s_e[w][head]);
+            for (int d = 4; d < 32; d <<= 1) l[n] += __shfl_xor_sync(~0u, l[n], d);
+            if (g == 0) s_m[warp][4 * n + t] = m[n], s_e[warp][4 * n + t] = e[n], s_l[warp][4 * n + t] = l[n];
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            l_all += s_l[w][head] * step_down(s_m[w][head], m_all);
-            keep[w] = step_down(s_e[w][head], e_all);
+            for (int j = 0; j < L::kQuads; ++j) out_w[(n * L::kQuads + j) * 32 + lane] = make_float4(o[n][j][0], o[n][j][1], o[n][j][2], o[n][j][3]);
         }
-        const uint32_t first_cta = unit_start / quota, last_cta = (unit_start + tiles - 1) / quota;
+        __syncthreads();
+        const uint32_t first_cta = owner(unit_start), last_cta = owner(unit_start + tiles - 1);
         const bool whole = first_cta == last_cta;
-        float *part = p.parts + (size_t(blockIdx.x) * 2 + (blockIdx.x == first_cta)) * kPartFloats<HD>;
-        // writes four elements of one column of a head
-        auto finish = [&](int quad, float4 x, float top, float etop, float sum) {
+        float *part = p.parts + (size_t(blockIdx.x) * 2 + (blockIdx.x == first_cta)) * kPartFloats<HD, NT>;
+        // quad f = n kQuads + j of lane (g, t): elements of head 4 n + t
+        auto finish = [&](int f, float4 x, float top, float etop, float sum) {
+            const int head = 4 * (f / L::kQuads) + t;
             if (head0 + head >= p.group) return;
             // 2^(etop - top) / sum, in two factors: either may be beyond binary32 where the output is not
             const float inverse = sum == 0.f ? 0.f : 1.f / sum;
@@ -437,37 +495,40 @@ __global__ void __launch_bounds__(kThreads, Layout<HD>::kResident) attention_ker
             const int h1 = power / 2;
             const float f1 = inverse * ldexpf(1.f, h1), f2 = ldexpf(1.f, power - h1);
             x = make_float4(x.x * f1 * f2, x.y * f1 * f2, x.z * f1 * f2, x.w * f1 * f2);
-            const int64_t out_at = int64_t(r) * a.out_stride + int64_t(kv * p.group + head0 + head) * HD + L::value_element(column, quad);
+            const int64_t out_at = int64_t(r) * a.out_stride + int64_t(kv * p.group + head0 + head) * HD + L::value_element(g, f % L::kQuads);
             if (a.ggml_type == JL_F16) {
                 const uint2 h = make_uint2(pack(__float2half_rn(x.x), __float2half_rn(x.y)), pack(__float2half_rn(x.z), __float2half_rn(x.w)));
                 *reinterpret_cast<uint2 *>(static_cast<__half *>(a.out) + out_at) = h;
             } else {
                 *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + out_at) = x;
             }
-            if (a.lse && quad == 0 && column == 0)
+            if (a.lse && f % L::kQuads == 0 && g == 0)
                 a.lse[int64_t(r) * a.heads + kv * p.group + head0 + head] = sum == 0.f ? -CUDART_INF_F : top * kLn2 + logf(sum);
         };
-#pragma unroll
-        for (int quad = tid >> 6; quad < HD / 32; quad += kThreads / 64) {
+        for (int f = warp; f < NT * L::kQuads; f += kWarps) {
+            const int head = 4 * (f / L::kQuads) + t;
+            float top = -CUDART_INF_F, etop = -CUDART_INF_F, sum = 0.f;
             float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
+            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w][head]), etop = fmaxf(etop, s_e[w][head]);
+#pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-                const float *src = reinterpret_cast<const float *>(smem) + w * L::kOut + quad * 256 + pair;
-                x.x += src[0] * keep[w], x.y += src[64] * keep[w], x.z += src[128] * keep[w], x.w += src[192] * keep[w];
+                const float keep = step_down(s_e[w][head], etop);
+                const float4 y = reinterpret_cast<const float4 *>(smem)[(w * NT * L::kQuads + f) * 32 + lane];
+                sum += s_l[w][head] * step_down(s_m[w][head], top);
+                x.x += y.x * keep, x.y += y.y * keep, x.z += y.z * keep, x.w += y.w * keep;
             }
             if (whole) {
-                finish(quad, x, m_all, e_all, l_all);
+                finish(f, x, top, etop, sum);
             } else {
-                float *dst = part + quad * 256 + pair;
-                dst[0] = x.x, dst[64] = x.y, dst[128] = x.z, dst[192] = x.w;
+                reinterpret_cast<float4 *>(part)[f * 32 + lane] = x;
+                if (f % L::kQuads == 0 && g == 0) {
+                    float *stats = part + kHeads * HD + head;
+                    stats[0] = top, stats[kHeads] = etop, stats[2 * kHeads] = sum;
+                }
             }
         }
         if (!whole) {
-            if (tid < 64 && column == 0) {
-                part[L::kOut + head] = m_all;
-                part[L::kOut + kHeads + head] = e_all;
-                part[L::kOut + 2 * kHeads + head] = l_all;
-            }
             __threadfence();
             __syncthreads();
             if (tid == 0) {
@@ -478,21 +539,23 @@ __global__ void __launch_bounds__(kThreads, Layout<HD>::kResident) attention_ker
             __syncthreads();
             if (last) {
                 const int n = int(last_cta - first_cta) + 1;
-                auto part_of = [&](int k) { return p.parts + (size_t(first_cta + k) * 2 + (k == 0)) * kPartFloats<HD>; };
-                float top = -CUDART_INF_F, etop = -CUDART_INF_F, sum = 0.f;
-                for (int k = 0; k < n; ++k) {
-                    top = fmaxf(top, __ldcg(part_of(k) + L::kOut + head));
-                    etop = fmaxf(etop, __ldcg(part_of(k) + L::kOut + kHeads + head));
-                }
-                for (int k = 0; k < n; ++k) sum += __ldcg(part_of(k) + L::kOut + 2 * kHeads + head) * step_down(__ldcg(part_of(k) + L::kOut + head), top);
-                for (int quad = tid >> 6; quad < HD / 32; quad += kThreads / 64) {
+                auto part_of = [&](int k) { return p.parts + (size_t(first_cta + k) * 2 + (k == 0)) * kPartFloats<HD, NT>; };
+                for (int f = warp; f < NT * L::kQuads; f += kWarps) {
+                    const int head = 4 * (f / L::kQuads) + t, at_stats = kHeads * HD + head;
+                    float top = -CUDART_INF_F, etop = -CUDART_INF_F, sum = 0.f;
                     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
                     for (int k = 0; k < n; ++k) {
-                        const float *src = part_of(k) + quad * 256 + pair;
-                        const float f = step_down(__ldcg(part_of(k) + L::kOut + kHeads + head), etop);
-                        x.x += __ldcg(src) * f, x.y += __ldcg(src + 64) * f, x.z += __ldcg(src + 128) * f, x.w += __ldcg(src + 192) * f;
+                        top = fmaxf(top, __ldcg(part_of(k) + at_stats));
+                        etop = fmaxf(etop, __ldcg(part_of(k) + at_stats + kHeads));
                     }
-                    finish(quad, x, top, etop, sum);
+                    for (int k = 0; k < n; ++k) {
+                        const float *from_part = part_of(k);
+                        const float keep = step_down(__ldcg(from_part + at_stats + kHeads), etop);
+                        const float4 y = __ldcg(reinterpret_cast<const float4 *>(from_part) + f * 32 + lane);
+                        sum += __ldcg(from_part + at_stats + 2 * kHeads) * step_down(__ldcg(from_part + at_stats), top);
+                        x.x += y.x * keep, x.y += y.y * keep, x.z += y.z * keep, x.w += y.w * keep;
+                    }
+                    finish(f, x, top, etop, sum);
                 }
             }
         }
@@ -503,7 +566,7 @@ __global__ void __launch_bounds__(kThreads, Layout<HD>::kResident) attention_ker
     }
 }
 
-template <int HD>
+template <int HD, int NT, bool PAGED16>
 cudaError_t launch(Params &p, const Kv8Scratch &s, int sm_count, cudaStream_t stream) {
     using L = Layout<HD>;
     static std::atomic<uint64_t> configured{0};  // a bit for each device
@@ -512,20 +575,29 @@ cudaError_t launch(Params &p, const Kv8Scratch &s, int sm_count, cudaStream_t st
     if (e != cudaSuccess) return e;
     const uint64_t bit = uint64_t(1) << (device & 63);
     if (device > 63 || !(configured.load(std::memory_order_acquire) & bit)) {
-        e = cudaFuncSetAttribute(attention_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
+        e = cudaFuncSetAttribute(attention_kernel<HD, NT, PAGED16>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
         if (e != cudaSuccess) return e;
         if (device <= 63) configured.fetch_or(bit, std::memory_order_release);
     }
-    // never more CTAs than tiles if every row were as long as the table is
+    // never more CTAs than tiles if every row were as long as the table is (a window may begin inside sixteen tokens)
     const jl_kv8_attention_args &a = p.a;
     int64_t most = int64_t(a.blocks_per_slot) * a.pages.block_tokens;
-    if (a.window > 0) most = most < a.window ? most : a.window;
+    if (a.window > 0) most = most < int64_t(a.window) + 15 ? most : int64_t(a.window) + 15;
+    p.head_tiles = (p.group + 4 * NT - 1) / (4 * NT);
+    p.units = p.head_tiles * a.pages.kv_heads;
     const int64_t tiles = (most + kTile - 1) / kTile * p.units * a.rows;
     const int grid = int(tiles < int64_t(sm_count) * L::kResident ? tiles : int64_t(sm_count) * L::kResident);
     p.arrivals = static_cast<unsigned *>(s.memory);
     p.parts = reinterpret_cast<float *>(static_cast<char *>(s.memory) + kKv8CounterBytes);
-    attention_kernel<HD><<<grid, kThreads, L::kBytes, stream>>>(p);
+    attention_kernel<HD, NT, PAGED16><<<grid, kThreads, L::kBytes, stream>>>(p);
     return cudaGetLastError();
+}
+
+template <int HD>
+cudaError_t launch_variant(Params &p, const Kv8Scratch &s, int sm_count, cudaStream_t stream) {
+    const bool paged16 = p.a.pages.block_tokens % 16 == 0;
+    if (p.group <= 4) return paged16 ? launch<HD, 1, true>(p, s, sm_count, stream) : launch<HD, 1, false>(p, s, sm_count, stream);
+    return paged16 ? launch<HD, 2, true>(p, s, sm_count, stream) : launch<HD, 2, false>(p, s, sm_count, stream);
 }
 
 constexpr int kMostResident = 4;
@@ -536,8 +608,8 @@ static_assert(Layout<64>::kResident <= kMostResident && Layout<128>::kResident <
 cudaError_t kv8_scratch_create(Kv8Scratch *s, int sm_count) {
     // two parts for each CTA of the largest grid, of the largest kind
     size_t part = 0;
-    for (const size_t n : {Layout<64>::kResident * kPartFloats<64>, Layout<96>::kResident * kPartFloats<96>, Layout<128>::kResident * kPartFloats<128>,
-                           Layout<192>::kResident * kPartFloats<192>, Layout<256>::kResident * kPartFloats<256>})
+    for (const size_t n : {Layout<64>::kResident * kPartFloats<64, 2>, Layout<96>::kResident * kPartFloats<96, 2>, Layout<128>::kResident * kPartFloats<128, 2>,
+                           Layout<192>::kResident * kPartFloats<192, 2>, Layout<256>::kResident * kPartFloats<256, 2>})
         part = part > n ? part : n;
     if (size_t(sm_count) * kMostResident * 4 > kKv8CounterBytes) return cudaErrorInvalidValue;
     cudaError_t e = cudaMalloc(&s->memory, kKv8CounterBytes + size_t(sm_count) * 2 * part * 4);
@@ -560,14 +632,12 @@ cudaError_t kv8_attention_launch(const jl_kv8_attention_args &a, const Kv8Scratc
     p.shift = 31 + bits;
     p.divide = (uint64_t(1) << p.shift) / uint64_t(a.pages.block_tokens) + 1;
     p.group = a.heads / a.pages.kv_heads;
-    p.head_tiles = (p.group + kHeads - 1) / kHeads;
-    p.units = p.head_tiles * a.pages.kv_heads;
     switch (a.pages.head_dim) {
-        case 64: return launch<64>(p, s, sm_count, stream);
-        case 96: return launch<96>(p, s, sm_count, stream);
-        case 128: return launch<128>(p, s, sm_count, stream);
-        case 192: return launch<192>(p, s, sm_count, stream);
-        default: return launch<256>(p, s, sm_count, stream);
+        case 64: return launch_variant<64>(p, s, sm_count, stream);
+        case 96: return launch_variant<96>(p, s, sm_count, stream);
+        case 128: return launch_variant<128>(p, s, sm_count, stream);
+        case 192: return launch_variant<192>(p, s, sm_count, stream);
+        default: return launch_variant<256>(p, s, sm_count, stream);
     }
 }
 
