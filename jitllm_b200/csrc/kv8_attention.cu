@@ -16,6 +16,7 @@
 #include <cuda_fp16.h>
 #include <math_constants.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "common.cuh"
@@ -28,6 +29,11 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kStep = 16;                // tokens that a warp takes at a time
 constexpr int kTile = kStep * kWarps;    // tokens of a tile
+constexpr uint32_t kMinTiles = 2;        // that a piece of a unit has at least
+constexpr uint32_t kLongQuota = 16;      // tiles for each CTA from which on lines are cut without regard to units
+constexpr int kRowsPerLane = 4;
+constexpr int kMostResident = 4;         // CTAs per SM
+constexpr int kMostSms = 160;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 
 // ---- layout of a stage in shared memory: 16 rows of keys, 16 rows of values, their scales, the mask of tokens that count -----------
@@ -39,12 +45,11 @@ struct Layout {
     static constexpr int kValues = kStep * kPitch, kScales = 2 * kValues, kMask = kScales + 2 * kStep * 4;
     static constexpr int kStage = kMask + 16;
     static constexpr int kStages = HD <= 96 ? 4 : 3;
-    static constexpr int kResident = HD <= 128 ? 4 : 2;  // CTAs per SM
     static constexpr int kRing = kStages * kStage;
     static constexpr int kQuads = HD / 32;               // groups of four elements that a lane has of a head's output
     static constexpr int kLoad = HD == 96 ? 1 : HD == 64 || HD == 192 ? 2 : 4;  // quads that one load of values brings
-    static constexpr int kBytes = kWarps * kRing;        // also holds the warps' outputs: 8 heads of HD floats each
-    static_assert(kRing >= 8 * HD * 4);
+    static constexpr int kBytes = kWarps * kRing;
+    static_assert(kStage >= 8 * HD * 4);                 // a stage also holds a warp's outputs of eight heads
 
     // where 16-byte piece c of row r is
     __device__ static int piece(int r, int c) {
@@ -67,6 +72,10 @@ struct Layout {
         else return (j >> 2) * 128 + g * 16 + (j & 3) * 4;
     }
 };
+
+// CTAs per SM: registers are the limit (accumulators and queries of NT groups of heads)
+template <int HD, int NT>
+constexpr int kResident = HD <= 96 || (HD == 128 && NT == 1) ? 4 : HD == 128 ? 3 : 2;
 
 struct Params {
     jl_kv8_attention_args a;
@@ -165,124 +174,230 @@ __device__ __forceinline__ uint32_t block_sum(uint32_t v, uint32_t *before, uint
 
 // NT: groups of four query heads. PAGED16: blocks are multiples of 16 tokens, so a step's sixteen rows lie behind one another.
 template <int HD, int NT, bool PAGED16>
-__global__ void __launch_bounds__(kThreads, Layout<HD>::kResident) attention_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, (kResident<HD, NT>)) attention_kernel(const Params p) {
     using L = Layout<HD>;
     constexpr int kHeads = 4 * NT;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ uint32_t warp_sums[kWarps], start_row, start_tile;
     __shared__ float s_m[kWarps][kHeads], s_e[kWarps][kHeads], s_l[kWarps][kHeads];
-    __shared__ int last;
+    __shared__ int s_last[2];
     const jl_kv8_attention_args &a = p.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int rows = a.token_count ? min(a.token_count[0], a.rows) : a.rows;
 
-    // ---- this CTA's piece of the line of tiles: [total b / CTAs, total (b + 1) / CTAs), a tile at least for each CTA that has one
-    uint32_t total = 0;
-    for (int base = 0; base < rows; base += kThreads) {
-        const int r = base + tid;
-        total += r < rows ? tiles_of(row_at(a, r)) * p.units : 0;
-    }
-    uint32_t before;
-    total = block_sum(total, &before, warp_sums);
-    if (total == 0) return;
-    const uint32_t ctas = min(gridDim.x, total);
-    if (blockIdx.x >= ctas) return;
-    uint32_t at = uint32_t(uint64_t(total) * blockIdx.x / ctas);
-    const uint32_t end = uint32_t(uint64_t(total) * (blockIdx.x + 1) / ctas);
-    auto owner = [&](uint32_t tile) { return uint32_t(((uint64_t(tile) + 1) * ctas - 1) / total); };
-    uint32_t front = 0;  // tiles in front of the rows from `base` on
-    for (int base = 0; base < rows; base += kThreads) {
-        const int r = base + tid;
-        const uint32_t mine = r < rows ? tiles_of(row_at(a, r)) * p.units : 0;
-        const uint32_t all = block_sum(mine, &before, warp_sums);
-        if (at >= front + before && at < front + before + mine) {
-            start_row = r;
-            start_tile = at - front - before;
+    // ---- what this CTA takes. Short lines: a piece of one unit, every unit cut into equal pieces of `quota` tiles at most, as
+    // many as there are CTAs. Long ones, and more rows than a warp holds: [at, end) of the line, cut without regard to units.
+    uint32_t at = 0, end = 0, piece = 0, pieces = 0, in_row = 0, ctas = gridDim.x, quota = 0, more_than = 0, total = 0;
+    int r = 0;
+    if (rows <= 32 * kRowsPerLane) {
+        uint32_t tiles[kRowsPerLane], mine = 0;
+#pragma unroll
+        for (int k = 0; k < kRowsPerLane; ++k) {
+            const int i = lane * kRowsPerLane + k;
+            tiles[k] = i < rows ? tiles_of(row_at(a, i)) : 0;
+            mine += tiles[k];
         }
-        front += all;
-        if (front > at) break;
+        total = __reduce_add_sync(~0u, mine) * p.units;
+        if (uint32_t(rows) * p.units <= ctas && total < ctas * kLongQuota) {
+            quota = max(kMinTiles, (total + ctas - 1) / ctas);
+            uint32_t n[kRowsPerLane], sum;
+            for (;;) {
+                sum = 0;
+#pragma unroll
+                for (int k = 0; k < kRowsPerLane; ++k) sum += n[k] = (tiles[k] + quota - 1) / quota;
+                if (__reduce_add_sync(~0u, sum) * p.units <= ctas) break;
+                quota += max(1u, quota / 8);
+            }
+            uint32_t before = sum;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const uint32_t o = __shfl_up_sync(~0u, before, d);
+                if (lane >= d) before += o;
+            }
+            if (blockIdx.x >= __shfl_sync(~0u, before, 31) * p.units) return;
+            before = (before - sum) * p.units;
+            uint32_t found = 0, found_in = 0, found_n = 0;
+#pragma unroll
+            for (int k = 0; k < kRowsPerLane; ++k) {
+                if (blockIdx.x >= before && blockIdx.x < before + n[k] * p.units) {
+                    found = lane * kRowsPerLane + k + 1;
+                    found_in = blockIdx.x - before;
+                    found_n = n[k];
+                }
+                before += n[k] * p.units;
+            }
+            const int from_lane = __ffs(__ballot_sync(~0u, found != 0)) - 1;
+            r = __shfl_sync(~0u, found, from_lane) - 1;
+            found_in = __shfl_sync(~0u, found_in, from_lane);
+            pieces = __shfl_sync(~0u, found_n, from_lane);
+            piece = found_in % pieces;
+            in_row = found_in / pieces;  // the unit, until enter() knows the row's tiles
+        }
     }
-    __syncthreads();
-    int r = start_row;
-    uint32_t in_row = start_tile;
+    if (pieces == 0) {
+        if (rows > 32 * kRowsPerLane) {
+            uint32_t mine = 0, before;
+            for (int i = tid; i < rows; i += kThreads) mine += tiles_of(row_at(a, i));
+            total = block_sum(mine, &before, warp_sums) * p.units;
+        }
+        if (total == 0) return;
+        ctas = min(ctas, total);
+        if (blockIdx.x >= ctas) return;
+        quota = total / ctas;
+        more_than = total % ctas;  // so many CTAs take one more
+        at = blockIdx.x * quota + min(blockIdx.x, more_than);
+        end = at + quota + (blockIdx.x < more_than);
+        uint32_t front = 0;  // tiles in front of the rows from `base` on
+        for (int base = 0; base < rows && front <= at; base += kThreads) {
+            uint32_t before;
+            const uint32_t mine = base + tid < rows ? tiles_of(row_at(a, base + tid)) * p.units : 0, all = block_sum(mine, &before, warp_sums);
+            if (at >= front + before && at < front + before + mine) {
+                start_row = base + tid;
+                start_tile = at - front - before;
+            }
+            front += all;
+        }
+        __syncthreads();
+        r = start_row;
+        in_row = start_tile;
+    }
+    auto owner = [&](uint32_t tile) {
+        const uint32_t longer = more_than * (quota + 1);
+        return tile < longer ? tile / (quota + 1) : more_than + (tile - longer) / quota;
+    };
 
     unsigned char *ring = smem + warp * L::kRing;
     const uint32_t ring_at = smem_u32(ring);
     const int bt = a.pages.block_tokens;
-    while (at < end) {
-        const Row row = row_at(a, r);
-        const uint32_t tiles = tiles_of(row);
-        const uint32_t unit = in_row / tiles, tile = in_row % tiles, take = min(tiles - tile, end - at);
-        const int kv = unit / p.head_tiles, head0 = (unit % p.head_tiles) * kHeads;  // head0: within the group
-        const uint32_t unit_start = at - tile;
-        // tokens of this piece, and the steps of them that this warp takes: i from 0 on, at token from + (warp + 4 i) 16
-        const uint32_t from = (row.first & ~15u) + tile * kTile, to = min(row.end, from + take * kTile);
-        const int steps = to > from ? int((to - from + kStep - 1) / kStep) : 0;
-        const int mine = steps > warp ? (steps - warp + kWarps - 1) / kWarps : 0;
-        const int32_t *line = a.block_table + int64_t(row.slot) * a.blocks_per_slot;
-        auto step_at = [&](int i) { return from + uint32_t(warp + i * kWarps) * kStep; };
-        auto block_of = [&](uint32_t j) { return uint32_t((j * p.divide) >> p.shift); };
 
-        // PAGED16: lane i looks up step 32 k + i of this warp, 32 steps ahead; where its codes and scales begin, or -1.
-        // Otherwise lanes i and i + 16 look up token i of a step, one step ahead.
-        int64_t code_at = -1, scale_at = -1;
-        int ahead;
-        auto look_up = [&](int i) {
-            if constexpr (PAGED16) return i + lane < mine ? line[block_of(step_at(i + lane))] : -1;
-            const uint32_t j = step_at(i) + (lane & 15);
-            return i < mine && j < to ? line[block_of(j)] : -1;
-        };
-        auto place = [&](int block, uint32_t j) {
-            const bool good = block >= 0 && block < a.pages.blocks;
-            const int64_t in_block = int64_t(kv) * bt + (j - block_of(j) * bt);
-            code_at = good ? block * a.pages.block_stride + in_block * HD : -1;
-            scale_at = block * a.pages.scale_stride + in_block;
-        };
-        auto issue = [&](int i) {
-            if (i < mine) {
-                const uint32_t stage = ring_at + uint32_t(i % L::kStages) * L::kStage, j0 = step_at(i);
-                unsigned mask = (j0 < row.first ? 0xffffu << (row.first - j0) : 0xffffu) & (to - j0 < 16 ? (1u << (to - j0)) - 1 : 0xffffu);
-                if constexpr (PAGED16) {
-                    if (i % 32 == 0) {
-                        place(ahead, step_at(i + lane));
-                        ahead = look_up(i + 32);
-                    }
-                    const int64_t code = __shfl_sync(~0u, code_at, i & 31), scale = __shfl_sync(~0u, scale_at, i & 31);
-                    if (code < 0) mask = 0;
-                    if (code >= 0) {
-                        const int8_t *k = a.pages.k + code + lane * 16, *v = a.pages.v + code + lane * 16;
-                        copy4(stage + L::kScales + 4 * lane, (lane < 16 ? a.pages.k_scale : a.pages.v_scale) + scale + (lane & 15));
-#pragma unroll
-                        for (int n = 0; n < HD / 32; ++n) {
-                            const int piece = n * 32 + lane;
-                            const uint32_t dst = stage + L::piece(piece / (HD / 16), piece % (HD / 16));
-                            copy16(dst, k + n * 512);
-                            copy16(dst + L::kValues, v + n * 512);
-                        }
-                    }
-                } else {
-                    place(ahead, j0 + (lane & 15));
-                    ahead = look_up(i + 1);
-                    mask &= __ballot_sync(~0u, code_at >= 0);
-                    if (code_at >= 0) copy4(stage + L::kScales + 4 * lane, (lane < 16 ? a.pages.k_scale : a.pages.v_scale) + scale_at);
+    // The segment under way: tiles [tile, tile + take) of a unit, tokens [from, to); `mine` steps of them are this warp's, step i at
+    // token from + (warp + 4 i) 16.
+    struct Segment {
+        uint32_t first, from, to, tiles, tile, take;
+        int kv, head0, mine;  // head0: within the group
+        const int32_t *line;
+    } seg;
+    auto enter = [&]() {
+        const Row row = row_at(a, r);
+        seg.tiles = tiles_of(row);
+        uint32_t unit = in_row;
+        if (pieces) {
+            seg.tile = seg.tiles * piece / pieces;
+            seg.take = seg.tiles * (piece + 1) / pieces - seg.tile;
+        } else {
+            unit = in_row / seg.tiles;
+            seg.tile = in_row % seg.tiles;
+            seg.take = min(seg.tiles - seg.tile, end - at);
+        }
+        seg.kv = unit / p.head_tiles;
+        seg.head0 = (unit % p.head_tiles) * kHeads;
+        seg.first = row.first;
+        seg.from = (row.first & ~15u) + seg.tile * kTile;
+        seg.to = min(row.end, seg.from + seg.take * kTile);
+        const int steps = seg.to > seg.from ? int((seg.to - seg.from + kStep - 1) / kStep) : 0;
+        seg.mine = steps > warp ? (steps - warp + kWarps - 1) / kWarps : 0;
+        seg.line = a.block_table + int64_t(row.slot) * a.blocks_per_slot;
+    };
+    auto step_at = [&](int i) { return seg.from + uint32_t(warp + i * kWarps) * kStep; };
+    auto block_of = [&](uint32_t j) { return uint32_t((j * p.divide) >> p.shift); };
+
+    // PAGED16: lane i looks up step 32 k + i of this warp, 32 steps ahead; where its codes and scales begin, or -1.
+    // Otherwise lanes i and i + 16 look up token i of a step, one step ahead.
+    int64_t code_at = -1, scale_at = -1;
+    int ahead;
+    auto look_up = [&](int i) {
+        if constexpr (PAGED16) return i + lane < seg.mine ? seg.line[block_of(step_at(i + lane))] : -1;
+        const uint32_t j = step_at(i) + (lane & 15);
+        return i < seg.mine && j < seg.to ? seg.line[block_of(j)] : -1;
+    };
+    auto place = [&](int block, uint32_t j) {
+        const bool good = block >= 0 && block < a.pages.blocks;
+        const int64_t in_block = int64_t(seg.kv) * bt + (j - block_of(j) * bt);
+        code_at = good ? block * a.pages.block_stride + in_block * HD : -1;
+        scale_at = block * a.pages.scale_stride + in_block;
+    };
+    auto issue = [&](int i) {
+        if (i < seg.mine) {
+            const uint32_t stage = ring_at + uint32_t(i % L::kStages) * L::kStage, j0 = step_at(i);
+            unsigned mask = (j0 < seg.first ? 0xffffu << (seg.first - j0) : 0xffffu) & (seg.to - j0 < 16 ? (1u << (seg.to - j0)) - 1 : 0xffffu);
+            if constexpr (PAGED16) {
+                if (i % 32 == 0) {
+                    place(ahead, step_at(i + lane));
+                    ahead = look_up(i + 32);
+                }
+                const int64_t code = __shfl_sync(~0u, code_at, i & 31), scale = __shfl_sync(~0u, scale_at, i & 31);
+                if (code < 0) mask = 0;
+                if (code >= 0) {
+                    const int8_t *k = a.pages.k + code + lane * 16, *v = a.pages.v + code + lane * 16;
+                    copy4(stage + L::kScales + 4 * lane, (lane < 16 ? a.pages.k_scale : a.pages.v_scale) + scale + (lane & 15));
 #pragma unroll
                     for (int n = 0; n < HD / 32; ++n) {
-                        const int piece = n * 32 + lane, row16 = piece / (HD / 16), c = piece % (HD / 16);
-                        const int64_t src = __shfl_sync(~0u, code_at, row16);
-                        const uint32_t dst = stage + L::piece(row16, c);
-                        if (src >= 0) {
-                            copy16(dst, a.pages.k + src + c * 16);
-                            copy16(dst + L::kValues, a.pages.v + src + c * 16);
-                        }
+                        const int piece = n * 32 + lane;
+                        const uint32_t dst = stage + L::piece(piece / (HD / 16), piece % (HD / 16));
+                        copy16(dst, k + n * 512);
+                        copy16(dst + L::kValues, v + n * 512);
                     }
                 }
-                if (lane == 0) *reinterpret_cast<unsigned *>(ring + (i % L::kStages) * L::kStage + L::kMask) = mask;
+            } else {
+                place(ahead, j0 + (lane & 15));
+                ahead = look_up(i + 1);
+                mask &= __ballot_sync(~0u, code_at >= 0);
+                if (code_at >= 0) copy4(stage + L::kScales + 4 * lane, (lane < 16 ? a.pages.k_scale : a.pages.v_scale) + scale_at);
+#pragma unroll
+                for (int n = 0; n < HD / 32; ++n) {
+                    const int piece = n * 32 + lane, row16 = piece / (HD / 16), c = piece % (HD / 16);
+                    const int64_t src = __shfl_sync(~0u, code_at, row16);
+                    const uint32_t dst = stage + L::piece(row16, c);
+                    if (src >= 0) {
+                        copy16(dst, a.pages.k + src + c * 16);
+                        copy16(dst + L::kValues, a.pages.v + src + c * 16);
+                    }
+                }
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
+            if (lane == 0) *reinterpret_cast<unsigned *>(ring + (i % L::kStages) * L::kStage + L::kMask) = mask;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto begin = [&]() {
+        enter();
         ahead = look_up(0);
 #pragma unroll
         for (int i = 0; i < L::kStages - 1; ++i) issue(i);
+    };
+
+    // Units of this CTA that others have a part of: two at most, its first and its last. Whether it was the last to arrive at one
+    // is asked for at once, and looked at when nothing else is left to do.
+    struct Shared {
+        int r, kv, head0;
+        uint32_t first, parts;
+    } shared[2];
+    int n_shared = 0;
+    bool arrived_last[2] = {false, false};  // thread 0
+
+    // quad f = n kQuads + j of lane (g, t): four elements of head 4 n + t
+    auto finish = [&](int f, int row, int kv, int head0, float4 x, float top, float etop, float sum) {
+        const int head = 4 * (f / L::kQuads) + t;
+        if (head0 + head >= p.group) return;
+        // 2^(etop - top) / sum, in two factors: either may be beyond binary32 where the output is not. etop is above top - 130 and
+        // below top + 116, since a weight's exponent is between -113 and 128.
+        const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+        const int power = sum == 0.f || !(fabsf(etop - top) < 200.f) ? 0 : int(etop - top), h1 = power / 2;
+        const float f1 = inverse * __int_as_float((127 + h1) << 23), f2 = __int_as_float((127 + power - h1) << 23);
+        x = make_float4(x.x * f1 * f2, x.y * f1 * f2, x.z * f1 * f2, x.w * f1 * f2);
+        const int64_t out_at = int64_t(row) * a.out_stride + int64_t(kv * p.group + head0 + head) * HD + L::value_element(g, f % L::kQuads);
+        if (a.ggml_type == JL_F16) {
+            const uint2 h = make_uint2(pack(__float2half_rn(x.x), __float2half_rn(x.y)), pack(__float2half_rn(x.z), __float2half_rn(x.w)));
+            *reinterpret_cast<uint2 *>(static_cast<__half *>(a.out) + out_at) = h;
+        } else {
+            *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + out_at) = x;
+        }
+        if (a.lse && f % L::kQuads == 0 && g == 0)
+            a.lse[int64_t(row) * a.heads + kv * p.group + head0 + head] = sum == 0.f ? -CUDART_INF_F : (top + __log2f(sum)) * kLn2;
+    };
+
+    begin();
+    for (;;) {
+        const int mine = seg.mine, kv = seg.kv, head0 = seg.head0;
 
         // ---- queries: column g of group n is part g & 1 of head 4 n + g / 2. Rotated, scaled, split.
         uint32_t q[NT][HD / 16][2];
@@ -293,8 +408,8 @@ __global__ void __launch_bounds__(kThreads, Layout<HD>::kResident) attention_ker
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const int head = head0 + 4 * n + (g >> 1);
-                float x[HD / 16][4], largest = 0.f;
-                bool finite = !outside;
+                float x[HD / 16][4];
+                uint32_t largest = outside ? 0x7f800000u : 0u;  // of the elements' magnitudes, as bits
                 const int64_t q_at = int64_t(r) * a.q_stride + int64_t(kv * p.group + head) * HD;
 #pragma unroll
                 for (int w = 0; w < HD / 16; ++w) {
@@ -316,16 +431,13 @@ __global__ void __launch_bounds__(kThreads, Layout<HD>::kResident) attention_ker
                     }
                     x[w][0] = v.x, x[w][1] = v.y, x[w][2] = v.z, x[w][3] = v.w;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        finite = finite && isfinite(x[w][k]);
-                        largest = fmaxf(largest, fabsf(x[w][k]));
-                    }
+                    for (int k = 0; k < 4; ++k) largest = max(largest, __float_as_uint(x[w][k]) & 0x7fffffffu);
                 }
-                largest = fmaxf(largest, __shfl_xor_sync(~0u, largest, 1));
-                largest = fmaxf(largest, __shfl_xor_sync(~0u, largest, 2));
-                finite = (__ballot_sync(~0u, finite) >> (lane & ~3) & 15) == 15;
+                largest = max(largest, __shfl_xor_sync(~0u, largest, 1));
+                largest = max(largest, __shfl_xor_sync(~0u, largest, 2));
+                const bool finite = largest < 0x7f800000u;
                 // 2^(14 - exponent of the largest), at most 2^126
-                const int shift = finite && largest > 0.f ? min(14 - (int(__float_as_uint(largest) >> 23) - 127), 126) : 0;
+                const int shift = finite ? min(14 - (int(largest >> 23) - 127), 126) : 0;
                 const float up = __uint_as_float(uint32_t(127 + shift) << 23);
 #pragma unroll
                 for (int w = 0; w < HD / 16; ++w)
@@ -336,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, Layout<HD>::kResident) attention_ker
                         q[n][w][k] = g & 1 ? rest : big;
                     }
                 // head 4 n + t is that of lanes with g = 2 t
-                factor[n] = __shfl_sync(~0u, finite ? a.scale * kLog2e * ldexpf(1.f, -shift) : CUDART_NAN_F, t * 8);
+                factor[n] = __shfl_sync(~0u, finite ? a.scale * kLog2e * __uint_as_float(uint32_t(127 - shift) << 23) : CUDART_NAN_F, t * 8);
             }
         }
 
@@ -469,10 +581,19 @@ __global__ void __launch_bounds__(kThreads, Layout<HD>::kResident) attention_ker
             }
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncwarp();
 
-        // ---- fold the warps. Outputs lie as [group][quad][lane], four elements of head t each.
-        __syncthreads();  // the rings are free
-        float4 *out_w = reinterpret_cast<float4 *>(smem) + warp * NT * L::kQuads * 32;
+        // ---- the next segment's first stages are on their way while this one's warps are folded, in the stage that they leave free.
+        // Outputs lie there as [group][quad][lane], four elements of head t each.
+        const int row = r;
+        // the CTAs that have a part of this unit
+        const uint32_t first_cta = pieces ? blockIdx.x - piece : owner(at - seg.tile), last_cta = pieces ? first_cta + pieces - 1 : owner(at - seg.tile + seg.tiles - 1);
+        at += seg.take;
+        in_row += seg.take;
+        if (in_row == seg.tiles * uint32_t(p.units)) ++r, in_row = 0;
+        const bool more = !pieces && at < end;
+        if (more) begin();
+        float4 *out_w = reinterpret_cast<float4 *>(ring + (L::kStages - 1) * L::kStage);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -482,29 +603,8 @@ __global__ void __launch_bounds__(kThreads, Layout<HD>::kResident) attention_ker
             for (int j = 0; j < L::kQuads; ++j) out_w[(n * L::kQuads + j) * 32 + lane] = make_float4(o[n][j][0], o[n][j][1], o[n][j][2], o[n][j][3]);
         }
         __syncthreads();
-        const uint32_t first_cta = owner(unit_start), last_cta = owner(unit_start + tiles - 1);
         const bool whole = first_cta == last_cta;
         float *part = p.parts + (size_t(blockIdx.x) * 2 + (blockIdx.x == first_cta)) * kPartFloats<HD, NT>;
-        // quad f = n kQuads + j of lane (g, t): elements of head 4 n + t
-        auto finish = [&](int f, float4 x, float top, float etop, float sum) {
-            const int head = 4 * (f / L::kQuads) + t;
-            if (head0 + head >= p.group) return;
-            // 2^(etop - top) / sum, in two factors: either may be beyond binary32 where the output is not
-            const float inverse = sum == 0.f ? 0.f : 1.f / sum;
-            const int power = sum == 0.f || etop == -CUDART_INF_F || top == -CUDART_INF_F ? 0 : int(etop - top);
-            const int h1 = power / 2;
-            const float f1 = inverse * ldexpf(1.f, h1), f2 = ldexpf(1.f, power - h1);
-            x = make_float4(x.x * f1 * f2, x.y * f1 * f2, x.z * f1 * f2, x.w * f1 * f2);
-            const int64_t out_at = int64_t(r) * a.out_stride + int64_t(kv * p.group + head0 + head) * HD + L::value_element(g, f % L::kQuads);
-            if (a.ggml_type == JL_F16) {
-                const uint2 h = make_uint2(pack(__float2half_rn(x.x), __float2half_rn(x.y)), pack(__float2half_rn(x.z), __float2half_rn(x.w)));
-                *reinterpret_cast<uint2 *>(static_cast<__half *>(a.out) + out_at) = h;
-            } else {
-                *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + out_at) = x;
-            }
-            if (a.lse && f % L::kQuads == 0 && g == 0)
-                a.lse[int64_t(r) * a.heads + kv * p.group + head0 + head] = sum == 0.f ? -CUDART_INF_F : top * kLn2 + logf(sum);
-        };
         for (int f = warp; f < NT * L::kQuads; f += kWarps) {
             const int head = 4 * (f / L::kQuads) + t;
             float top = -CUDART_INF_F, etop = -CUDART_INF_F, sum = 0.f;
@@ -514,12 +614,12 @@ __global__ void __launch_bounds__(kThreads, Layout<HD>::kResident) attention_ker
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
                 const float keep = step_down(s_e[w][head], etop);
-                const float4 y = reinterpret_cast<const float4 *>(smem)[(w * NT * L::kQuads + f) * 32 + lane];
+                const float4 y = reinterpret_cast<const float4 *>(smem + w * L::kRing + (L::kStages - 1) * L::kStage)[f * 32 + lane];
                 sum += s_l[w][head] * step_down(s_m[w][head], top);
                 x.x += y.x * keep, x.y += y.y * keep, x.z += y.z * keep, x.w += y.w * keep;
             }
             if (whole) {
-                finish(f, x, top, etop, sum);
+                finish(f, row, kv, head0, x, top, etop, sum);
             } else {
                 reinterpret_cast<float4 *>(part)[f * 32 + lane] = x;
                 if (f % L::kQuads == 0 && g == 0) {
@@ -528,41 +628,101 @@ __global__ void __launch_bounds__(kThreads, Layout<HD>::kResident) attention_ker
                 }
             }
         }
+        __syncthreads();  // the part is written, the fold's stage is free
         if (!whole) {
-            __threadfence();
-            __syncthreads();
+            const unsigned others = last_cta - first_cta;
             if (tid == 0) {
-                const unsigned others = last_cta - first_cta;
-                last = atomicInc(p.arrivals + first_cta, others) == others;  // the last one to come sets it back to zero
                 __threadfence();
+                const bool is_last = atomicInc(p.arrivals + first_cta, others) == others;  // the last one to come sets it back to zero
+                if (n_shared == 0) arrived_last[0] = is_last;
+                else arrived_last[1] = is_last;
             }
-            __syncthreads();
-            if (last) {
-                const int n = int(last_cta - first_cta) + 1;
-                auto part_of = [&](int k) { return p.parts + (size_t(first_cta + k) * 2 + (k == 0)) * kPartFloats<HD, NT>; };
-                for (int f = warp; f < NT * L::kQuads; f += kWarps) {
-                    const int head = 4 * (f / L::kQuads) + t, at_stats = kHeads * HD + head;
-                    float top = -CUDART_INF_F, etop = -CUDART_INF_F, sum = 0.f;
-                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int k = 0; k < n; ++k) {
-                        top = fmaxf(top, __ldcg(part_of(k) + at_stats));
-                        etop = fmaxf(etop, __ldcg(part_of(k) + at_stats + kHeads));
-                    }
-                    for (int k = 0; k < n; ++k) {
-                        const float *from_part = part_of(k);
-                        const float keep = step_down(__ldcg(from_part + at_stats + kHeads), etop);
-                        const float4 y = __ldcg(reinterpret_cast<const float4 *>(from_part) + f * 32 + lane);
-                        sum += __ldcg(from_part + at_stats + 2 * kHeads) * step_down(__ldcg(from_part + at_stats), top);
-                        x.x += y.x * keep, x.y += y.y * keep, x.z += y.z * keep, x.w += y.w * keep;
-                    }
-                    finish(f, x, top, etop, sum);
-                }
+            const Shared unit = {row, kv, head0, first_cta, others + 1};
+            if (n_shared == 0) shared[0] = unit;
+            else shared[1] = unit;
+            ++n_shared;
+        }
+        if (!more) break;
+    }
+
+    // ---- join the units that this CTA came last to
+    if (n_shared == 0) return;
+    if (tid == 0) {
+        s_last[0] = arrived_last[0];
+        s_last[1] = arrived_last[1];
+        __threadfence();
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        if (u >= n_shared || !s_last[u]) continue;
+        const Shared &unit = shared[u];
+        const int n = int(unit.parts);
+        auto part_of = [&](int k) { return p.parts + (size_t(unit.first + k) * 2 + (k == 0)) * kPartFloats<HD, NT>; };
+        // maxima and sums: thread i has head i mod heads of every (threads / heads)-th part
+        const int my_head = tid % kHeads;
+        float top = -CUDART_INF_F, etop = -CUDART_INF_F, sum = 0.f;
+#pragma unroll 4
+        for (int k = tid / kHeads; k < n; k += kThreads / kHeads) {
+            const float *stats = part_of(k) + kHeads * HD + my_head;
+            top = fmaxf(top, __ldcg(stats));
+            etop = fmaxf(etop, __ldcg(stats + kHeads));
+        }
+#pragma unroll
+        for (int d = kHeads; d < 32; d <<= 1) {
+            top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+            etop = fmaxf(etop, __shfl_xor_sync(~0u, etop, d));
+        }
+        __syncthreads();  // what was kept here before has been read
+        if (lane < kHeads) s_m[warp][lane] = top, s_e[warp][lane] = etop;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w][my_head]), etop = fmaxf(etop, s_e[w][my_head]);
+        float *keep = reinterpret_cast<float *>(smem);  // [part][head]
+#pragma unroll 4
+        for (int k = tid / kHeads; k < n; k += kThreads / kHeads) {
+            const float *stats = part_of(k) + kHeads * HD + my_head;
+            sum += __ldcg(stats + 2 * kHeads) * step_down(__ldcg(stats), top);
+            keep[k * kHeads + my_head] = step_down(__ldcg(stats + kHeads), etop);
+        }
+#pragma unroll
+        for (int d = kHeads; d < 32; d <<= 1) sum += __shfl_xor_sync(~0u, sum, d);
+        if (lane < kHeads) s_l[warp][lane] = sum;
+        __syncthreads();
+        // outputs: a warp has every fourth part
+        constexpr int kUnroll = NT * L::kQuads <= 4 ? 4 : NT * L::kQuads <= 8 ? 2 : 1;
+        float4 x[NT * L::kQuads];
+#pragma unroll
+        for (int f = 0; f < NT * L::kQuads; ++f) x[f] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll kUnroll
+        for (int k = warp; k < n; k += kWarps) {
+            const float4 *src = reinterpret_cast<const float4 *>(part_of(k)) + lane;
+#pragma unroll
+            for (int f = 0; f < NT * L::kQuads; ++f) {
+                const float4 y = __ldcg(src + f * 32);
+                const float w = keep[k * kHeads + 4 * (f / L::kQuads) + t];
+                x[f].x += y.x * w, x[f].y += y.y * w, x[f].z += y.z * w, x[f].w += y.w * w;
             }
         }
-        __syncthreads();  // shared memory is free for the next unit
-        at += take;
-        in_row += take;
-        if (in_row == tiles * uint32_t(p.units)) ++r, in_row = 0;
+        float4 *warp_out = reinterpret_cast<float4 *>(smem + kMostResident * kMostSms * kHeads * 4);  // behind `keep`
+        static_assert(kMostResident * kMostSms * kHeads * 4 + kWarps * NT * HD * 16 <= L::kBytes);
+#pragma unroll
+        for (int f = 0; f < NT * L::kQuads; ++f) warp_out[(warp * NT * L::kQuads + f) * 32 + lane] = x[f];
+        __syncthreads();
+        for (int f = warp; f < NT * L::kQuads; f += kWarps) {
+            const int head = 4 * (f / L::kQuads) + t;
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+            float all = 0.f, head_top = -CUDART_INF_F, head_etop = -CUDART_INF_F;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float4 z = warp_out[(w * NT * L::kQuads + f) * 32 + lane];
+                y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
+                all += s_l[w][head];
+                head_top = fmaxf(head_top, s_m[w][head]), head_etop = fmaxf(head_etop, s_e[w][head]);
+            }
+            finish(f, unit.r, unit.kv, unit.head0, y, head_top, head_etop, all);
+        }
+        __syncthreads();
     }
 }
 
@@ -586,7 +746,7 @@ cudaError_t launch(Params &p, const Kv8Scratch &s, int sm_count, cudaStream_t st
     p.head_tiles = (p.group + 4 * NT - 1) / (4 * NT);
     p.units = p.head_tiles * a.pages.kv_heads;
     const int64_t tiles = (most + kTile - 1) / kTile * p.units * a.rows;
-    const int grid = int(tiles < int64_t(sm_count) * L::kResident ? tiles : int64_t(sm_count) * L::kResident);
+    const int grid = int(tiles < int64_t(sm_count) * kResident<HD, NT> ? tiles : int64_t(sm_count) * kResident<HD, NT>);
     p.arrivals = static_cast<unsigned *>(s.memory);
     p.parts = reinterpret_cast<float *>(static_cast<char *>(s.memory) + kKv8CounterBytes);
     attention_kernel<HD, NT, PAGED16><<<grid, kThreads, L::kBytes, stream>>>(p);
@@ -600,19 +760,15 @@ cudaError_t launch_variant(Params &p, const Kv8Scratch &s, int sm_count, cudaStr
     return paged16 ? launch<HD, 2, true>(p, s, sm_count, stream) : launch<HD, 2, false>(p, s, sm_count, stream);
 }
 
-constexpr int kMostResident = 4;
-static_assert(Layout<64>::kResident <= kMostResident && Layout<128>::kResident <= kMostResident && Layout<256>::kResident <= kMostResident);
-
+static_assert(kMostSms * kMostResident * 4 <= kKv8CounterBytes);
 }  // namespace
 
 cudaError_t kv8_scratch_create(Kv8Scratch *s, int sm_count) {
     // two parts for each CTA of the largest grid, of the largest kind
-    size_t part = 0;
-    for (const size_t n : {Layout<64>::kResident * kPartFloats<64, 2>, Layout<96>::kResident * kPartFloats<96, 2>, Layout<128>::kResident * kPartFloats<128, 2>,
-                           Layout<192>::kResident * kPartFloats<192, 2>, Layout<256>::kResident * kPartFloats<256, 2>})
-        part = part > n ? part : n;
-    if (size_t(sm_count) * kMostResident * 4 > kKv8CounterBytes) return cudaErrorInvalidValue;
-    cudaError_t e = cudaMalloc(&s->memory, kKv8CounterBytes + size_t(sm_count) * 2 * part * 4);
+    const int part = std::max({kResident<64, 2> * kPartFloats<64, 2>, kResident<96, 2> * kPartFloats<96, 2>, kResident<128, 1> * kPartFloats<128, 1>,
+                               kResident<128, 2> * kPartFloats<128, 2>, kResident<192, 2> * kPartFloats<192, 2>, kResident<256, 2> * kPartFloats<256, 2>});
+    if (sm_count > kMostSms) return cudaErrorInvalidValue;  // more CTAs than there are counters, or than a join has room for
+    cudaError_t e = cudaMalloc(&s->memory, kKv8CounterBytes + size_t(sm_count) * 2 * part * sizeof(float));
     if (e == cudaSuccess) e = cudaMemset(s->memory, 0, kKv8CounterBytes);
     if (e == cudaSuccess) e = cudaDeviceSynchronize();  // the memset is over before a launch on any stream
     return e;
