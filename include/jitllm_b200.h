@@ -312,7 +312,7 @@ int32_t jl_kv8_workspace_free(jl_ctx *ctx, jl_kv8_workspace *ws);
 /* Block table and slot map. Sequence r holds held[r] tokens and gets added[r] more. Sequences are served in order: one whose
  * tokens need new blocks takes them from free_blocks, from *cursor on, and their ids follow the ids of its blocks in its row of
  * the table; the table's other entries are left as they are. A sequence is refused (nothing of it changes, its tokens get
- * position and place -1) if held or added is negative, if it would grow beyond blocks_per_slot blocks, if its tokens do not all
+ * position and place -1) if held or added is negative, if it would grow beyond blocks_per_slot blocks or 2^31 - 1 tokens, if its tokens do not all
  * lie within `capacity`, or if the blocks it needs, together with those that the sequences before it need (refused for lack of
  * blocks or not), are more than there are.
  * New tokens are numbered through, sequence after sequence: token offsets[r] + i is sequence r's token at position held[r] + i

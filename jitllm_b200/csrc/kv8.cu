@@ -2,155 +2,358 @@
 #include <cuda_fp16.h>
 #include <math_constants.h>
 
+#include <algorithm>
+#include <atomic>
+
 #include "common.cuh"
 #include "kv8.cuh"
 
 namespace jl {
 namespace {
 
-constexpr int kMapThreads = 1024;
+// ---- block tables and slot maps -----------------------------------------------------------------
+//
+// With t_r = max(added_r, 0) and its running sum, need_r = ceil((held_r + added_r) / B) - ceil(held_r / B) blocks and their running
+// sum, everything a token or a new block needs is known: token i belongs to the last sequence whose sum begins at or below i, block
+// number b to the last sequence whose blocks begin at or below b. Every CTA works both sums out for itself (at most 8192
+// sequences, 64 KB from L2) and keeps them in shared memory; then tokens and blocks are dealt out evenly, whatever the
+// sequences' lengths. So there is one launch and nothing to wait for between CTAs. What may be an input and an output at once
+// (lengths, cursor) is written by the CTA that is through last.
 
-// Sum over the block's threads up to and including this one; the whole sum goes to every thread.
-__device__ long long block_inclusive(long long v, long long *warp_sums, long long *total) {
+constexpr int kMapThreads = 512;
+constexpr int kMapWarps = kMapThreads / 32;
+constexpr int kMapTokens = 1024;  // tokens of capacity for each CTA, up to one CTA per SM
+
+struct MapParams {
+    jl_kv8_map_args a;
+    uint64_t divide;  // j / block_tokens = j * divide >> shift for j < 2^31
+    int shift;
+    bool in_place;
+    unsigned *arrivals;
+};
+
+__device__ __forceinline__ uint32_t add_saturated(uint32_t a, uint32_t b) { return a + b < a ? ~0u : a + b; }
+
+// Saturated sums of v over the threads in front of this one; that of all threads in *all.
+__device__ uint32_t exclusive_sum(uint32_t v, uint32_t *warp_sums, uint32_t *all) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t s = v;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const long long o = __shfl_up_sync(~0u, v, d);
-        if (lane >= d) v += o;
+        const uint32_t o = __shfl_up_sync(~0u, s, d);
+        if (lane >= d) s = add_saturated(s, o);
     }
+    const uint32_t in_front = __shfl_up_sync(~0u, s, 1);
     __syncthreads();
-    if (lane == 31) warp_sums[warp] = v;
+    if (lane == 31) warp_sums[warp] = s;
     __syncthreads();
-    long long before = 0, all = 0;
-    for (int w = 0; w < int(blockDim.x) / 32; ++w) {
-        if (w < warp) before += warp_sums[w];
-        all += warp_sums[w];
+    uint32_t w = lane < kMapWarps ? warp_sums[lane] : 0;
+#pragma unroll
+    for (int d = 1; d < kMapWarps; d <<= 1) {
+        const uint32_t o = __shfl_up_sync(~0u, w, d);
+        if (lane >= d) w = add_saturated(w, o);
     }
-    *total = all;
-    return before + v;
+    const uint32_t before = __shfl_sync(~0u, w, max(warp - 1, 0));
+    *all = __shfl_sync(~0u, w, kMapWarps - 1);
+    return add_saturated(warp ? before : 0, lane ? in_front : 0);
 }
 
-// One CTA walks the sequences, a thread each, and writes a sequence's blocks and tokens one after the other.
-__global__ void __launch_bounds__(kMapThreads) map_kernel(jl_kv8_map_args a) {
-    __shared__ long long warp_sums[kMapThreads / 32];
-    const int tid = threadIdx.x;
-    const int cursor = a.cursor[0];
-    const long long free_blocks = cursor < 0 || cursor > a.free_count ? 0 : a.free_count - cursor;
-    const long long room = (long long)a.blocks_per_slot * a.block_tokens;
-    long long tokens = 0, asked = 0, taken = 0, refused = 0;
-    for (int base = 0; base < a.sequences; base += kMapThreads) {
-        const int r = base + tid;
-        const bool here = r < a.sequences;
-        const long long held = here ? a.held[r] : 0, added = here ? a.added[r] : 0;
-        const long long count = added > 0 ? added : 0;
-        long long all;
-        const long long end = tokens + block_inclusive(count, warp_sums, &all);
-        tokens += all;
-        const bool bad = held < 0 || added < 0 || held + added > room || end > a.capacity;
-        const long long have = bad ? 0 : (held + a.block_tokens - 1) / a.block_tokens;
-        const long long need = bad ? 0 : (held + added + a.block_tokens - 1) / a.block_tokens - have;
-        const long long block_end = asked + block_inclusive(need, warp_sums, &all);
-        asked += all;
-        const bool served = !bad && (need == 0 || block_end <= free_blocks);
-        block_inclusive(here && !served, warp_sums, &all);
-        refused += all;
-        block_inclusive(served ? need : 0, warp_sums, &all);
-        taken += all;
-        if (!here) continue;
-        int32_t *row = a.block_table + (size_t)r * a.blocks_per_slot;
-        if (served)
-            for (long long j = 0; j < need; ++j) row[have + j] = a.free_blocks[cursor + block_end - need + j];
-        a.lengths[r] = int32_t(served ? held + added : held);
-        const long long start = end - count;
-        if (a.offsets) {
-            a.offsets[r] = int32_t(min(start, (long long)INT32_MAX));
-            if (r == a.sequences - 1) a.offsets[r + 1] = int32_t(min(end, (long long)INT32_MAX));
-        }
-        for (long long i = 0; i < count && start + i < a.capacity; ++i) {
-            const long long t = start + i, pos = served ? held + i : -1;
-            const int block = pos < 0 ? -1 : row[pos / a.block_tokens];
-            a.slot_map[t] = block < 0 ? -1 : (long long)block * a.block_tokens + pos % a.block_tokens;
-            if (a.positions) a.positions[t] = int32_t(pos);
-            if (a.token_slots) a.token_slots[t] = r;
-        }
+// The last r in [low, high] with starts[r] <= x; starts ascend and starts[low] <= x.
+__device__ __forceinline__ int last_at_most(const uint32_t *starts, int low, int high, uint32_t x) {
+    while (low < high) {
+        const int middle = (low + high + 1) >> 1;
+        if (starts[middle] <= x) low = middle;
+        else high = middle - 1;
     }
+    return low;
+}
+
+__global__ void __launch_bounds__(kMapThreads) map_kernel(const MapParams p) {
+    extern __shared__ uint32_t smem[];
+    __shared__ uint32_t warp_sums[32], s_taken, s_refused;
+    __shared__ bool s_last;
+    const jl_kv8_map_args &a = p.a;
+    const int n = a.sequences, tid = threadIdx.x;
+    uint32_t *token_start = smem, *block_start = smem + n;
+    int32_t *kept = reinterpret_cast<int32_t *>(smem + 2 * n);  // held; below 0: the sequence is refused
+    auto block_of = [&](uint32_t position) { return uint32_t((uint64_t(position) * p.divide) >> p.shift); };
+    auto blocks_for = [&](uint32_t tokens) { return tokens ? block_of(tokens - 1) + 1 : 0; };
+
+    if (tid == 0) s_taken = s_refused = 0;
+    const int cursor = a.cursor[0];
+    const uint32_t free_blocks = cursor < 0 || cursor > a.free_count ? 0 : a.free_count - cursor;
+    const int64_t room = min(int64_t(a.blocks_per_slot) * a.block_tokens, int64_t(INT32_MAX));
+    // each thread has sequences [from, to)
+    const int each = (n + kMapThreads - 1) / kMapThreads, from = min(n, tid * each), to = min(n, from + each);
+    uint32_t sum = 0, tokens, asked;
+    for (int r = from; r < to; ++r) sum = add_saturated(sum, uint32_t(max(a.added[r], 0)));
+    uint32_t at = exclusive_sum(sum, warp_sums, &tokens);
+    sum = 0;
+    for (int r = from; r < to; ++r) {
+        const int held = a.held[r], added = a.added[r];
+        token_start[r] = at;
+        at = add_saturated(at, uint32_t(max(added, 0)));
+        const bool bad = held < 0 || added < 0 || int64_t(held) + added > room || at > uint32_t(a.capacity);
+        const uint32_t need = bad ? 0 : blocks_for(held + added) - blocks_for(held);
+        kept[r] = bad ? -1 : held;
+        block_start[r] = need;
+        sum = add_saturated(sum, need);
+    }
+    at = exclusive_sum(sum, warp_sums, &asked);
+    uint32_t taken = 0, refused = 0;
+    for (int r = from; r < to; ++r) {
+        const uint32_t need = block_start[r], block_end = add_saturated(at, need);
+        block_start[r] = at;
+        at = block_end;
+        if (kept[r] >= 0 && need != 0) {
+            if (block_end <= free_blocks) taken = block_end;
+            else kept[r] = -1;
+        }
+        refused += kept[r] < 0;
+    }
+    if (taken) atomicMax(&s_taken, taken);
+    if (refused) atomicAdd(&s_refused, refused);
     __syncthreads();
+    taken = s_taken;
+
+    // ---- new blocks: numbers 0 .. taken - 1, all of sequences that are served
+    const int step = gridDim.x * kMapThreads;
+    for (uint32_t b = blockIdx.x * kMapThreads + tid; b < taken; b += step) {
+        const int r = last_at_most(block_start, 0, n - 1, b);
+        a.block_table[int64_t(r) * a.blocks_per_slot + blocks_for(kept[r]) + (b - block_start[r])] = a.free_blocks[cursor + b];
+    }
+    // ---- new tokens
+    const uint32_t written = min(tokens, uint32_t(a.capacity));
+    int low = 0;
+    for (uint32_t i = blockIdx.x * kMapThreads + tid; i < written; i += step) {
+        const int r = low = last_at_most(token_start, low, n - 1, i);
+        int32_t position = -1;
+        int64_t place = -1;
+        if (kept[r] >= 0) {
+            position = int32_t(uint32_t(kept[r]) + (i - token_start[r]));
+            const uint32_t index = block_of(position), have = blocks_for(kept[r]);
+            // an entry below `have` is one that was there and that nobody writes
+            const int block = index < have ? a.block_table[int64_t(r) * a.blocks_per_slot + index] : a.free_blocks[cursor + block_start[r] + (index - have)];
+            if (block >= 0) place = int64_t(block) * a.block_tokens + (uint32_t(position) - index * a.block_tokens);
+        }
+        a.slot_map[i] = place;
+        if (a.positions) a.positions[i] = position;
+        if (a.token_slots) a.token_slots[i] = r;
+    }
+    // ---- what goes by sequences
+    if (a.offsets)
+        for (int r = blockIdx.x * kMapThreads + tid; r <= n; r += step) a.offsets[r] = int32_t(min(r < n ? token_start[r] : tokens, 0x7fffffffu));
+    auto length = [&](int r) { return kept[r] < 0 ? a.held[r] : kept[r] + a.added[r]; };
+    if (!p.in_place)
+        for (int r = blockIdx.x * kMapThreads + tid; r < n; r += step) a.lengths[r] = length(r);
+    bool last = blockIdx.x == 0;
+    if (p.in_place && gridDim.x > 1) {
+        __syncthreads();  // this CTA has read all it reads of held and cursor
+        if (tid == 0) {
+            __threadfence();
+            s_last = atomicInc(p.arrivals, gridDim.x - 1) == gridDim.x - 1;
+            __threadfence();
+        }
+        __syncthreads();
+        last = s_last;
+    } else if (p.in_place) {
+        __syncthreads();
+    }
+    if (!last) return;
+    if (p.in_place)
+        for (int r = tid; r < n; r += kMapThreads) a.lengths[r] = length(r);
     if (tid == 0) {
         a.cursor_out[0] = cursor + int32_t(taken);
-        a.result[0] = int32_t(min(tokens, (long long)a.capacity));
+        a.result[0] = int32_t(written);
         a.result[1] = int32_t(taken);
-        a.result[2] = int32_t(refused);
-        a.result[3] = int32_t(min(asked, (long long)INT32_MAX));
+        a.result[2] = int32_t(s_refused);
+        a.result[3] = int32_t(min(asked, 0x7fffffffu));
     }
 }
 
-__device__ __forceinline__ double load_as_double(const void *p, bool f16, int64_t i) {
-    return f16 ? double(__half2float(static_cast<const __half *>(p)[i])) : double(static_cast<const float *>(p)[i]);
-}
+// ---- append -------------------------------------------------------------------------------------
+//
+// A row (a token's keys or values of one head) is held by D / 8 lanes, eight elements each, so a warp has one to four rows and reads
+// them in 16-byte pieces. Codes are those of the unrounded values, so that they are a function of the row alone: with y = 127 x / max |x|
+// in binary32 (off by less than 5.3e-5: a rotation 2.5, the maximum as much, quotient and product 1 each, of 127 * 2^-24), a row
+// that has an element within 2^-13 of the border of two codes is done again in 64 bits, and so are rows whose largest element is
+// infinite, NaN or close to 2^-100. That is a row in thirty.
 
-// A warp per token, head and side, in 64 bits throughout.
-__global__ void __launch_bounds__(256) append_kernel(jl_kv8_append_args a) {
-    const int lane = threadIdx.x & 31;
-    const int64_t unit = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-    const int heads = a.pages.kv_heads, d = a.pages.head_dim;
-    const int64_t t = unit / (2 * heads);
-    const int side = int(unit % 2), head = int(unit % (2 * heads)) / 2;
+constexpr int kAppendThreads = 256;
+
+template <typename T>
+struct Eight;
+template <>
+struct Eight<float> {
+    float4 lo, hi;
+    __device__ void load(const float *p) {
+        lo = __ldcs(reinterpret_cast<const float4 *>(p));
+        hi = __ldcs(reinterpret_cast<const float4 *>(p) + 1);
+    }
+    __device__ void get(float (&x)[8]) const { x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w, x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w; }
+};
+template <>
+struct Eight<__half> {
+    uint4 v;
+    __device__ void load(const __half *p) { v = __ldcs(reinterpret_cast<const uint4 *>(p)); }
+    __device__ void get(float (&x)[8]) const {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+            x[2 * i] = f.x, x[2 * i + 1] = f.y;
+        }
+    }
+};
+
+struct AppendParams {
+    jl_kv8_append_args a;
+    uint64_t divide;  // j / block_tokens = j * divide >> shift for j < 2^31
+    int shift;
+};
+
+template <int HD, typename T>
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendParams p) {
+    constexpr int kLanes = HD <= 64 ? 8 : HD <= 128 ? 16 : 32;  // HD / 8 of them have elements
+    const jl_kv8_append_args &a = p.a;
+    const int sub = threadIdx.x % kLanes;
+    const uint32_t heads = a.pages.kv_heads, row = blockIdx.x * uint32_t(kAppendThreads / kLanes) + threadIdx.x / kLanes;  // rows: token, side, head
+    const uint32_t t = row / (2 * heads), in_token = row - t * 2 * heads;
+    const bool values = in_token >= heads;
+    const uint32_t head = values ? in_token - heads : in_token;
     const int count = a.token_count ? min(a.token_count[0], a.tokens) : a.tokens;
-    if (t >= count) return;
-    const int64_t place = a.slot_map[t];
-    if (place < 0 || place >= int64_t(a.pages.blocks) * a.pages.block_tokens) return;
-    const void *src = side ? a.v : a.k;
-    const int64_t at = t * (side ? a.v_stride : a.k_stride) + int64_t(head) * d;
-    const bool f16 = a.ggml_type == JL_F16, turn = side == 0 && a.rope_cos;
+    const bool here = int64_t(t) < count, mine = here && sub < HD / 8;
+    const int64_t place = here ? a.slot_map[t] : -1;
+
+    Eight<T> raw = {};
+    if (mine) raw.load(static_cast<const T *>(values ? a.v : a.k) + t * (values ? a.v_stride : a.k_stride) + head * HD + sub * 8);
+    const bool turn = here && !values && a.rope_cos;
     const int pos = turn ? a.positions[t] : 0;
     const bool outside = turn && (pos < 0 || pos >= a.rope_rows);
-    double x[4][2], most = 0;
-    bool good = !outside;
+    float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (turn && !outside && mine) {
+        c = *reinterpret_cast<const float4 *>(a.rope_cos + int64_t(pos) * (HD / 2) + sub * 4);
+        s = *reinterpret_cast<const float4 *>(a.rope_sin + int64_t(pos) * (HD / 2) + sub * 4);
+    }
+    const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
+    float in[8], x[8];
+    raw.get(in);
+    uint32_t bits = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int e = 2 * (lane + 32 * i);
-        x[i][0] = x[i][1] = 0;
-        if (e >= d) continue;
-        double p = load_as_double(src, f16, at + e), q = load_as_double(src, f16, at + e + 1);
-        if (turn && !outside) {
-            const int64_t angle = int64_t(pos) * (d / 2) + e / 2;
-            const double c = a.rope_cos[angle], s = a.rope_sin[angle], rotated = p * c - q * s;
-            q = p * s + q * c;
-            p = rotated;
+        x[2 * i] = turn ? in[2 * i] * cs[i] - in[2 * i + 1] * sn[i] : in[2 * i];
+        x[2 * i + 1] = turn ? in[2 * i] * sn[i] + in[2 * i + 1] * cs[i] : in[2 * i + 1];
+        bits = max(bits, max(__float_as_uint(x[2 * i]) & 0x7fffffffu, __float_as_uint(x[2 * i + 1]) & 0x7fffffffu));
+    }
+#pragma unroll
+    for (int d = kLanes / 2; d; d >>= 1) bits = max(bits, __shfl_xor_sync(~0u, bits, d));
+    const float most = __uint_as_float(bits), up = 127.f / most;
+    bool again = outside || !(most >= 0x1p-99f && most < CUDART_INF_F);
+    float y[8];
+    int code[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        y[i] = x[i] * up;
+        const float whole = rintf(y[i]);
+        again = again || fabsf(fabsf(y[i] - whole) - 0.5f) < 0x1p-13f;
+        code[i] = int(whole);
+    }
+    float scale = most / 127.f;
+    // whether any lane of the row says so
+    const unsigned says = __ballot_sync(~0u, again && here);
+    if (says) {
+        const unsigned row_lanes = kLanes == 32 ? ~0u : ((1u << (kLanes & 31)) - 1) << (threadIdx.x & 31 & ~(kLanes - 1));
+        double exact[8], largest = 0;
+        bool good = !outside;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const double u = in[2 * i], w = in[2 * i + 1];
+            exact[2 * i] = turn ? u * double(cs[i]) - w * double(sn[i]) : u;
+            exact[2 * i + 1] = turn ? u * double(sn[i]) + w * double(cs[i]) : w;
+            good = good && isfinite(exact[2 * i]) && isfinite(exact[2 * i + 1]);
+            largest = fmax(largest, fmax(fabs(exact[2 * i]), fabs(exact[2 * i + 1])));
         }
-        x[i][0] = p;
-        x[i][1] = q;
-        good = good && isfinite(p) && isfinite(q);
-        most = fmax(most, fmax(fabs(p), fabs(q)));
-    }
-    good = __all_sync(~0u, good);
+        good = (__ballot_sync(~0u, good) & row_lanes) == row_lanes;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) most = fmax(most, __shfl_xor_sync(~0u, most, o));
-    const bool some = good && most >= 0x1p-100;
-    const int64_t block = place / a.pages.block_tokens, row = int64_t(head) * a.pages.block_tokens + place % a.pages.block_tokens;
-    int8_t *codes = (side ? a.pages.v : a.pages.k) + block * a.pages.block_stride + row * d;
+        for (int d = kLanes / 2; d; d >>= 1) largest = fmax(largest, __shfl_xor_sync(~0u, largest, d));
+        if (says & row_lanes) {
+            const bool some = good && largest >= 0x1p-100;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int e = 2 * (lane + 32 * i);
-        if (e >= d) continue;
-        const int lo = some ? int(rint(x[i][0] * 127.0 / most)) : 0, hi = some ? int(rint(x[i][1] * 127.0 / most)) : 0;
-        *reinterpret_cast<char2 *>(codes + e) = make_char2(char(lo), char(hi));
+            for (int i = 0; i < 8; ++i) code[i] = some ? int(rint(exact[i] * 127.0 / largest)) : 0;
+            scale = good ? (some ? float(largest / 127.0) : 0.f) : CUDART_NAN_F;
+        }
     }
-    if (lane == 0)
-        (side ? a.pages.v_scale : a.pages.k_scale)[block * a.pages.scale_stride + row] = good ? (some ? float(most / 127.0) : 0.f) : CUDART_NAN_F;
+    if (!mine || place < 0 || place >= int64_t(a.pages.blocks) * a.pages.block_tokens) return;
+    // a place may be beyond 31 bits
+    const int64_t block = place < 0x7fffffff ? int64_t((uint64_t(place) * p.divide) >> p.shift) : place / a.pages.block_tokens;
+    const int64_t at = int64_t(head) * a.pages.block_tokens + (place - block * a.pages.block_tokens);
+    int8_t *to = (values ? a.pages.v : a.pages.k) + block * a.pages.block_stride + at * HD + sub * 8;
+    uint2 packed;
+    packed.x = (code[0] & 255) | (code[1] & 255) << 8 | (code[2] & 255) << 16 | code[3] << 24;
+    packed.y = (code[4] & 255) | (code[5] & 255) << 8 | (code[6] & 255) << 16 | code[7] << 24;
+    *reinterpret_cast<uint2 *>(to) = packed;
+    if (sub == 0) (values ? a.pages.v_scale : a.pages.k_scale)[block * a.pages.scale_stride + at] = scale;
+}
+
+template <int HD>
+cudaError_t append_launch(const AppendParams &p, cudaStream_t stream) {
+    constexpr int kLanes = HD <= 64 ? 8 : HD <= 128 ? 16 : 32;
+    const int64_t rows = int64_t(p.a.tokens) * p.a.pages.kv_heads * 2;
+    const unsigned grid = unsigned((rows * kLanes + kAppendThreads - 1) / kAppendThreads);
+    if (p.a.ggml_type == JL_F16) append_kernel<HD, __half><<<grid, kAppendThreads, 0, stream>>>(p);
+    else append_kernel<HD, float><<<grid, kAppendThreads, 0, stream>>>(p);
+    return cudaGetLastError();
 }
 
 }  // namespace
 
-cudaError_t kv8_map_launch(const jl_kv8_map_args &a, const Kv8Scratch &, int, cudaStream_t stream) {
-    map_kernel<<<1, kMapThreads, 0, stream>>>(a);
+void kv8_division(int divisor, uint64_t *divide, int *shift) {
+    int bits = 0;
+    while ((int64_t(1) << bits) < divisor) ++bits;
+    // floor(2^(31 + bits) / n) + 1 gives exact quotients of 31-bit numbers by n <= 2^bits (Granlund and Montgomery 1994)
+    *shift = 31 + bits;
+    *divide = (uint64_t(1) << *shift) / uint64_t(divisor) + 1;
+}
+
+cudaError_t kv8_map_launch(const jl_kv8_map_args &a, const Kv8Scratch &s, int sm_count, cudaStream_t stream) {
+    MapParams p = {};
+    p.a = a;
+    kv8_division(a.block_tokens, &p.divide, &p.shift);
+    p.in_place = a.lengths == a.held || a.cursor_out == a.cursor;
+    p.arrivals = reinterpret_cast<unsigned *>(static_cast<char *>(s.memory) + kKv8MapCounter);
+    const size_t bytes = size_t(a.sequences) * 12;
+    if (bytes > 40 * 1024) {  // 48 KB with what the kernel has besides
+        static std::atomic<uint64_t> configured{0};  // a bit for each device
+        const cudaError_t e = kv8_allow_shared(reinterpret_cast<const void *>(map_kernel), 8192 * 12, configured);
+        if (e != cudaSuccess) return e;
+    }
+    const int grid = std::max(1, std::min(sm_count, int((int64_t(std::max(a.capacity, a.sequences)) + kMapTokens - 1) / kMapTokens)));
+    map_kernel<<<grid, kMapThreads, bytes, stream>>>(p);
     return cudaGetLastError();
 }
 
 cudaError_t kv8_append_launch(const jl_kv8_append_args &a, int, cudaStream_t stream) {
-    const int64_t warps = int64_t(a.tokens) * a.pages.kv_heads * 2;
-    append_kernel<<<unsigned((warps + 7) / 8), 256, 0, stream>>>(a);
-    return cudaGetLastError();
+    AppendParams p = {};
+    p.a = a;
+    kv8_division(a.pages.block_tokens, &p.divide, &p.shift);
+    switch (a.pages.head_dim) {
+        case 64: return append_launch<64>(p, stream);
+        case 96: return append_launch<96>(p, stream);
+        case 128: return append_launch<128>(p, stream);
+        case 192: return append_launch<192>(p, stream);
+        default: return append_launch<256>(p, stream);
+    }
+}
+
+cudaError_t kv8_allow_shared(const void *kernel, int bytes, std::atomic<uint64_t> &configured) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = uint64_t(1) << (device & 63);
+    if (device <= 63 && (configured.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && device <= 63) configured.fetch_or(bit, std::memory_order_release);
+    return e;
 }
 
 }  // namespace jl

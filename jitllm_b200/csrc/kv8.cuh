@@ -3,6 +3,8 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "../../include/jitllm_b200.h"
 
 namespace jl {
@@ -13,12 +15,17 @@ int kv8_check_append(const jl_kv8_append_args *a, char *message, size_t n);
 int kv8_check_attention(const jl_kv8_attention_args *a, char *message, size_t n);
 
 // The device half of a jl_kv8_workspace: counters that are zero between launches, then the attention's parts.
-constexpr size_t kKv8CounterBytes = 16384;
+constexpr size_t kKv8CounterBytes = 16384, kKv8MapCounter = kKv8CounterBytes - 128;
 struct Kv8Scratch {
     void *memory = nullptr;
 };
 cudaError_t kv8_scratch_create(Kv8Scratch *s, int sm_count);
 void kv8_scratch_free(Kv8Scratch *s);
+
+// Constants with which j / divisor = j * divide >> shift for j < 2^31; divisor at most 2^31.
+void kv8_division(int divisor, uint64_t *divide, int *shift);
+// Lets a kernel have so many bytes of dynamic shared memory on the current device; `configured` has a bit for each device.
+cudaError_t kv8_allow_shared(const void *kernel, int bytes, std::atomic<uint64_t> &configured);
 
 // Arguments that have passed the checks, on the current device.
 cudaError_t kv8_map_launch(const jl_kv8_map_args &a, const Kv8Scratch &s, int sm_count, cudaStream_t stream);

@@ -730,15 +730,8 @@ template <int HD, int NT, bool PAGED16>
 cudaError_t launch(Params &p, const Kv8Scratch &s, int sm_count, cudaStream_t stream) {
     using L = Layout<HD>;
     static std::atomic<uint64_t> configured{0};  // a bit for each device
-    int device = 0;
-    cudaError_t e = cudaGetDevice(&device);
+    const cudaError_t e = kv8_allow_shared(reinterpret_cast<const void *>(attention_kernel<HD, NT, PAGED16>), L::kBytes, configured);
     if (e != cudaSuccess) return e;
-    const uint64_t bit = uint64_t(1) << (device & 63);
-    if (device > 63 || !(configured.load(std::memory_order_acquire) & bit)) {
-        e = cudaFuncSetAttribute(attention_kernel<HD, NT, PAGED16>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
-        if (e != cudaSuccess) return e;
-        if (device <= 63) configured.fetch_or(bit, std::memory_order_release);
-    }
     // never more CTAs than tiles if every row were as long as the table is (a window may begin inside sixteen tokens)
     const jl_kv8_attention_args &a = p.a;
     int64_t most = int64_t(a.blocks_per_slot) * a.pages.block_tokens;
@@ -760,7 +753,7 @@ cudaError_t launch_variant(Params &p, const Kv8Scratch &s, int sm_count, cudaStr
     return paged16 ? launch<HD, 2, true>(p, s, sm_count, stream) : launch<HD, 2, false>(p, s, sm_count, stream);
 }
 
-static_assert(kMostSms * kMostResident * 4 <= kKv8CounterBytes);
+static_assert(kMostSms * kMostResident * 4 <= kKv8MapCounter);
 }  // namespace
 
 cudaError_t kv8_scratch_create(Kv8Scratch *s, int sm_count) {
@@ -782,11 +775,7 @@ void kv8_scratch_free(Kv8Scratch *s) {
 cudaError_t kv8_attention_launch(const jl_kv8_attention_args &a, const Kv8Scratch &s, int sm_count, cudaStream_t stream) {
     Params p = {};
     p.a = a;
-    int bits = 0;
-    while ((int64_t(1) << bits) < a.pages.block_tokens) ++bits;
-    // floor(2^(31 + bits) / n) + 1 gives exact quotients of 31-bit numbers by n <= 2^bits (Granlund and Montgomery 1994)
-    p.shift = 31 + bits;
-    p.divide = (uint64_t(1) << p.shift) / uint64_t(a.pages.block_tokens) + 1;
+    kv8_division(a.pages.block_tokens, &p.divide, &p.shift);
     p.group = a.heads / a.pages.kv_heads;
     switch (a.pages.head_dim) {
         case 64: return launch_variant<64>(p, s, sm_count, stream);

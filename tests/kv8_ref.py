@@ -16,7 +16,7 @@ def map_ref(held, added, table, free, cursor, block, capacity, token_slots, posi
         h, a = int(held[r]), int(added[r])
         start = tokens
         tokens += max(a, 0)
-        bad = h < 0 or a < 0 or h + a > per * block or tokens > capacity
+        bad = h < 0 or a < 0 or h + a > min(per * block, 2**31 - 1) or tokens > capacity
         have = 0 if bad else -(-h // block)
         need = 0 if bad else -(-(h + a) // block) - have
         asked += need

@@ -76,7 +76,8 @@ class _Map:
 
 @pytest.mark.parametrize("n,block,most_added,short,seed", [
     (1, 16, 1, False, 0), (1, 1, 5, False, 1), (2, 16, 40, False, 2), (31, 16, 3, True, 3), (33, 7, 50, False, 4), (257, 16, 1, False, 5),
-    (1000, 32, 90, True, 6), (1025, 16, 2, False, 7), (8192, 16, 9, False, 8), (8192, 64, 40, True, 9), (5, 65536, 100000, False, 10), (3, 16, 300000, False, 11)])
+    (1000, 32, 90, True, 6), (1025, 16, 2, False, 7), (3413, 16, 3, False, 12), (3500, 16, 1, True, 13), (4096, 32, 5, False, 14), (4097, 16, 1, False, 15),
+    (8192, 16, 9, False, 8), (8192, 64, 40, True, 9), (5, 65536, 100000, False, 10), (3, 16, 300000, False, 11)])
 def test_map_of_random_batches(ws, n, block, most_added, short, seed):
     rng = np.random.default_rng(seed)
     held = rng.integers(0, 4 * block, n)
