@@ -22,13 +22,13 @@ namespace {
 
 constexpr int kMapThreads = 512;
 constexpr int kMapWarps = kMapThreads / 32;
-constexpr int kMapTokens = 1024;  // tokens of capacity for each CTA, up to one CTA per SM
 
 struct MapParams {
     jl_kv8_map_args a;
     uint64_t divide;  // j / block_tokens = j * divide >> shift for j < 2^31
     int shift;
     bool in_place;
+    bool wide;        // the token arrays are 16-byte aligned
     unsigned *arrivals;
 };
 
@@ -68,6 +68,8 @@ __device__ __forceinline__ int last_at_most(const uint32_t *starts, int low, int
     return low;
 }
 
+// EACH: tokens in a row that a thread has. One where there are few, four (a wide store for each array) where there are many.
+template <int EACH>
 __global__ void __launch_bounds__(kMapThreads) map_kernel(const MapParams p) {
     extern __shared__ uint32_t smem[];
     __shared__ uint32_t warp_sums[32], s_taken, s_refused;
@@ -83,14 +85,16 @@ __global__ void __launch_bounds__(kMapThreads) map_kernel(const MapParams p) {
     const int cursor = a.cursor[0];
     const uint32_t free_blocks = cursor < 0 || cursor > a.free_count ? 0 : a.free_count - cursor;
     const int64_t room = min(int64_t(a.blocks_per_slot) * a.block_tokens, int64_t(INT32_MAX));
-    // each thread has sequences [from, to)
-    const int each = (n + kMapThreads - 1) / kMapThreads, from = min(n, tid * each), to = min(n, from + each);
+    // each thread has sequences [from, to), an odd number of them, so that a warp's threads meet in no bank
+    const int each = (n + kMapThreads - 1) / kMapThreads | 1, from = min(n, tid * each), to = min(n, from + each);
+    for (int r = tid; r < n; r += kMapThreads) block_start[r] = a.added[r], kept[r] = a.held[r];
+    __syncthreads();
     uint32_t sum = 0, tokens, asked;
-    for (int r = from; r < to; ++r) sum = add_saturated(sum, uint32_t(max(a.added[r], 0)));
+    for (int r = from; r < to; ++r) sum = add_saturated(sum, uint32_t(max(int32_t(block_start[r]), 0)));
     uint32_t at = exclusive_sum(sum, warp_sums, &tokens);
     sum = 0;
     for (int r = from; r < to; ++r) {
-        const int held = a.held[r], added = a.added[r];
+        const int held = kept[r], added = int32_t(block_start[r]);
         token_start[r] = at;
         at = add_saturated(at, uint32_t(max(added, 0)));
         const bool bad = held < 0 || added < 0 || int64_t(held) + added > room || at > uint32_t(a.capacity);
@@ -111,8 +115,10 @@ __global__ void __launch_bounds__(kMapThreads) map_kernel(const MapParams p) {
         }
         refused += kept[r] < 0;
     }
-    if (taken) atomicMax(&s_taken, taken);
-    if (refused) atomicAdd(&s_refused, refused);
+    taken = __reduce_max_sync(~0u, taken);
+    refused = __reduce_add_sync(~0u, refused);
+    if ((tid & 31) == 0 && taken) atomicMax(&s_taken, taken);
+    if ((tid & 31) == 0 && refused) atomicAdd(&s_refused, refused);
     __syncthreads();
     taken = s_taken;
 
@@ -125,20 +131,39 @@ __global__ void __launch_bounds__(kMapThreads) map_kernel(const MapParams p) {
     // ---- new tokens
     const uint32_t written = min(tokens, uint32_t(a.capacity));
     int low = 0;
-    for (uint32_t i = blockIdx.x * kMapThreads + tid; i < written; i += step) {
-        const int r = low = last_at_most(token_start, low, n - 1, i);
-        int32_t position = -1;
-        int64_t place = -1;
-        if (kept[r] >= 0) {
-            position = int32_t(uint32_t(kept[r]) + (i - token_start[r]));
-            const uint32_t index = block_of(position), have = blocks_for(kept[r]);
-            // an entry below `have` is one that was there and that nobody writes
-            const int block = index < have ? a.block_table[int64_t(r) * a.blocks_per_slot + index] : a.free_blocks[cursor + block_start[r] + (index - have)];
-            if (block >= 0) place = int64_t(block) * a.block_tokens + (uint32_t(position) - index * a.block_tokens);
+    for (uint32_t i0 = EACH * (blockIdx.x * kMapThreads + tid); i0 < written; i0 += EACH * step) {
+        int r = low = last_at_most(token_start, low, n - 1, i0);
+        int slot[EACH], position[EACH];
+        int64_t place[EACH];
+#pragma unroll
+        for (int k = 0; k < EACH; ++k) {
+            const uint32_t i = i0 + k;
+            if (k && i < written && r < n - 1 && token_start[r + 1] <= i) r = last_at_most(token_start, r + 1, n - 1, i);
+            slot[k] = r;
+            position[k] = -1;
+            place[k] = -1;
+            if (i < written && kept[r] >= 0) {
+                position[k] = int32_t(uint32_t(kept[r]) + (i - token_start[r]));
+                const uint32_t index = block_of(position[k]), have = blocks_for(kept[r]);
+                // an entry below `have` is one that was there and that nobody writes
+                const int block = index < have ? a.block_table[int64_t(r) * a.blocks_per_slot + index] : a.free_blocks[cursor + block_start[r] + (index - have)];
+                if (block >= 0) place[k] = int64_t(block) * a.block_tokens + (uint32_t(position[k]) - index * a.block_tokens);
+            }
         }
-        a.slot_map[i] = place;
-        if (a.positions) a.positions[i] = position;
-        if (a.token_slots) a.token_slots[i] = r;
+        if (EACH == 4 && p.wide && i0 + 4 <= written) {
+            reinterpret_cast<longlong2 *>(a.slot_map + i0)[0] = make_longlong2(place[0], place[EACH / 4]);
+            reinterpret_cast<longlong2 *>(a.slot_map + i0)[1] = make_longlong2(place[EACH / 2], place[EACH - 1]);
+            if (a.positions) *reinterpret_cast<int4 *>(a.positions + i0) = make_int4(position[0], position[EACH / 4], position[EACH / 2], position[EACH - 1]);
+            if (a.token_slots) *reinterpret_cast<int4 *>(a.token_slots + i0) = make_int4(slot[0], slot[EACH / 4], slot[EACH / 2], slot[EACH - 1]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < EACH; ++k)
+                if (i0 + k < written) {
+                    a.slot_map[i0 + k] = place[k];
+                    if (a.positions) a.positions[i0 + k] = position[k];
+                    if (a.token_slots) a.token_slots[i0 + k] = slot[k];
+                }
+        }
     }
     // ---- what goes by sequences
     if (a.offsets)
@@ -171,13 +196,26 @@ __global__ void __launch_bounds__(kMapThreads) map_kernel(const MapParams p) {
     }
 }
 
+template <int EACH>
+cudaError_t map_launch(const MapParams &p, int64_t most, int ctas, cudaStream_t stream) {
+    const size_t bytes = size_t(p.a.sequences) * 12;
+    if (bytes > 40 * 1024) {  // 48 KB with what the kernel has besides
+        static std::atomic<uint64_t> configured{0};  // a bit for each device
+        const cudaError_t e = kv8_allow_shared(reinterpret_cast<const void *>(map_kernel<EACH>), 8192 * 12, configured);
+        if (e != cudaSuccess) return e;
+    }
+    const int64_t grid = (most + EACH * kMapThreads - 1) / (EACH * kMapThreads);
+    map_kernel<EACH><<<int(std::max(int64_t(1), std::min(int64_t(ctas), grid))), kMapThreads, bytes, stream>>>(p);
+    return cudaGetLastError();
+}
+
 // ---- append -------------------------------------------------------------------------------------
 //
 // A row (a token's keys or values of one head) is held by D / 8 lanes, eight elements each, so a warp has one to four rows and reads
-// them in 16-byte pieces. Codes are those of the unrounded values, so that they are a function of the row alone: with y = 127 x / max |x|
-// in binary32 (off by less than 5.3e-5: a rotation 2.5, the maximum as much, quotient and product 1 each, of 127 * 2^-24), a row
-// that has an element within 2^-13 of the border of two codes is done again in 64 bits, and so are rows whose largest element is
-// infinite, NaN or close to 2^-100. That is a row in thirty.
+// them in 16-byte pieces. Codes are those of the unrounded values, so that they are a function of the row alone: with 127 x / max |x|
+// in binary32 (off by less than 7e-5: a rotation 2.5, the maximum as much, the quotient 4, of 127 * 2^-24), a row that has an
+// element within 2^-13 of the border of two codes is done again in 64 bits, and so are rows whose largest element is infinite, NaN,
+// above 2^125 or close to 2^-100. That is a row in thirty.
 
 constexpr int kAppendThreads = 256;
 
@@ -208,8 +246,8 @@ struct Eight<__half> {
 
 struct AppendParams {
     jl_kv8_append_args a;
-    uint64_t divide;  // j / block_tokens = j * divide >> shift for j < 2^31
-    int shift;
+    uint64_t divide, divide_rows;  // j / block_tokens = j * divide >> shift for j < 2^31; the same for rows of a token
+    int shift, shift_rows;
 };
 
 template <int HD, typename T>
@@ -218,7 +256,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
     const jl_kv8_append_args &a = p.a;
     const int sub = threadIdx.x % kLanes;
     const uint32_t heads = a.pages.kv_heads, row = blockIdx.x * uint32_t(kAppendThreads / kLanes) + threadIdx.x / kLanes;  // rows: token, side, head
-    const uint32_t t = row / (2 * heads), in_token = row - t * 2 * heads;
+    const uint32_t t = uint32_t((uint64_t(row) * p.divide_rows) >> p.shift_rows), in_token = row - t * 2 * heads;
     const bool values = in_token >= heads;
     const uint32_t head = values ? in_token - heads : in_token;
     const int count = a.token_count ? min(a.token_count[0], a.tokens) : a.tokens;
@@ -247,18 +285,17 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
     }
 #pragma unroll
     for (int d = kLanes / 2; d; d >>= 1) bits = max(bits, __shfl_xor_sync(~0u, bits, d));
-    const float most = __uint_as_float(bits), up = 127.f / most;
-    bool again = outside || !(most >= 0x1p-99f && most < CUDART_INF_F);
-    float y[8];
-    int code[8];
+    const float most = __uint_as_float(bits), up = __fdividef(127.f, most), magic = 12582912.f;  // 1.5 * 2^23: a sum's low byte is the code
+    float border = 0.f;
+    uint32_t code[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        y[i] = x[i] * up;
-        const float whole = rintf(y[i]);
-        again = again || fabsf(fabsf(y[i] - whole) - 0.5f) < 0x1p-13f;
-        code[i] = int(whole);
+        const float y = fmaf(x[i], up, magic);
+        border = fmaxf(border, fabsf(fmaf(x[i], up, magic - y)));
+        code[i] = __float_as_uint(y);
     }
-    float scale = most / 127.f;
+    const bool again = outside || !(most >= 0x1p-99f && most < 0x1p125f) || border > 0.5f - 0x1p-13f;
+    float scale = most * (1.f / 127.f);
     // whether any lane of the row says so
     const unsigned says = __ballot_sync(~0u, again && here);
     if (says) {
@@ -279,7 +316,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
         if (says & row_lanes) {
             const bool some = good && largest >= 0x1p-100;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) code[i] = some ? int(rint(exact[i] * 127.0 / largest)) : 0;
+            for (int i = 0; i < 8; ++i) code[i] = some ? uint32_t(int(rint(exact[i] * 127.0 / largest))) : 0;
             scale = good ? (some ? float(largest / 127.0) : 0.f) : CUDART_NAN_F;
         }
     }
@@ -289,8 +326,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
     const int64_t at = int64_t(head) * a.pages.block_tokens + (place - block * a.pages.block_tokens);
     int8_t *to = (values ? a.pages.v : a.pages.k) + block * a.pages.block_stride + at * HD + sub * 8;
     uint2 packed;
-    packed.x = (code[0] & 255) | (code[1] & 255) << 8 | (code[2] & 255) << 16 | code[3] << 24;
-    packed.y = (code[4] & 255) | (code[5] & 255) << 8 | (code[6] & 255) << 16 | code[7] << 24;
+    packed.x = __byte_perm(__byte_perm(code[0], code[1], 0x0040), __byte_perm(code[2], code[3], 0x0040), 0x5410);
+    packed.y = __byte_perm(__byte_perm(code[4], code[5], 0x0040), __byte_perm(code[6], code[7], 0x0040), 0x5410);
     *reinterpret_cast<uint2 *>(to) = packed;
     if (sub == 0) (values ? a.pages.v_scale : a.pages.k_scale)[block * a.pages.scale_stride + at] = scale;
 }
@@ -319,23 +356,19 @@ cudaError_t kv8_map_launch(const jl_kv8_map_args &a, const Kv8Scratch &s, int sm
     MapParams p = {};
     p.a = a;
     kv8_division(a.block_tokens, &p.divide, &p.shift);
+    auto aligned = [](const void *x) { return reinterpret_cast<uintptr_t>(x) % 16 == 0; };
+    p.wide = aligned(a.slot_map) && aligned(a.positions) && aligned(a.token_slots);
     p.in_place = a.lengths == a.held || a.cursor_out == a.cursor;
     p.arrivals = reinterpret_cast<unsigned *>(static_cast<char *>(s.memory) + kKv8MapCounter);
-    const size_t bytes = size_t(a.sequences) * 12;
-    if (bytes > 40 * 1024) {  // 48 KB with what the kernel has besides
-        static std::atomic<uint64_t> configured{0};  // a bit for each device
-        const cudaError_t e = kv8_allow_shared(reinterpret_cast<const void *>(map_kernel), 8192 * 12, configured);
-        if (e != cudaSuccess) return e;
-    }
-    const int grid = std::max(1, std::min(sm_count, int((int64_t(std::max(a.capacity, a.sequences)) + kMapTokens - 1) / kMapTokens)));
-    map_kernel<<<grid, kMapThreads, bytes, stream>>>(p);
-    return cudaGetLastError();
+    const int64_t most = std::max(a.capacity, a.sequences);
+    return most <= int64_t(sm_count) * kMapThreads ? map_launch<1>(p, most, sm_count, stream) : map_launch<4>(p, most, 2 * sm_count, stream);
 }
 
 cudaError_t kv8_append_launch(const jl_kv8_append_args &a, int, cudaStream_t stream) {
     AppendParams p = {};
     p.a = a;
     kv8_division(a.pages.block_tokens, &p.divide, &p.shift);
+    kv8_division(2 * a.pages.kv_heads, &p.divide_rows, &p.shift_rows);
     switch (a.pages.head_dim) {
         case 64: return append_launch<64>(p, stream);
         case 96: return append_launch<96>(p, stream);

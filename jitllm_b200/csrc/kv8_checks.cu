@@ -77,8 +77,8 @@ int kv8_check_append(const jl_kv8_append_args *a, char *message, size_t n) {
     int rc = check_pages(a->pages, message, n);
     if (rc) return rc;
     const int64_t row = int64_t(a->pages.kv_heads) * a->pages.head_dim;
-    KV8_REQUIRE(a->tokens >= 0 && int64_t(a->tokens) * a->pages.kv_heads <= 1 << 30, JL_ERR_INVALID,
-                "tokens must not be negative, and tokens times heads at most 2^30, got %d tokens of %d heads", a->tokens, a->pages.kv_heads);
+    KV8_REQUIRE(a->tokens >= 0 && int64_t(a->tokens) * a->pages.kv_heads <= 1 << 29, JL_ERR_INVALID,
+                "tokens must not be negative, and tokens times heads at most 2^29, got %d tokens of %d heads", a->tokens, a->pages.kv_heads);
     if ((rc = check_rows("k", a->k, a->k_stride, row, a->ggml_type, message, n))) return rc;
     if ((rc = check_rows("v", a->v, a->v_stride, row, a->ggml_type, message, n))) return rc;
     if ((rc = check_rope(a->rope_cos, a->rope_sin, a->positions, a->rope_rows, message, n))) return rc;
