@@ -2305,7 +2305,7 @@ int32_t jl_kv8_map(jl_ctx *ctx, jl_kv8_workspace *ws, const jl_kv8_map_args *arg
     if (rc) return fail(ctx, rc, "%s", message);
     JL_REQUIRE(ctx, owns(ctx, ws), JL_ERR_INVALID, "the workspace is not one of this context's");
     DeviceGuard guard(ctx->device);
-    const cudaError_t e = kv8_map_launch(*args, ws->scratch, ctx->sm_count, static_cast<cudaStream_t>(stream));
+    const cudaError_t e = kv8_map_launch(*args, ws->scratch, {ctx->sm_count, ctx->use_pdl, static_cast<cudaStream_t>(stream)});
     if (e != cudaSuccess) return fail(ctx, JL_ERR_CUDA, "block map launch failed: %s", cudaGetErrorString(e));
     ctx->counters.kernel_launches++;
     return JL_OK;
@@ -2318,7 +2318,7 @@ int32_t jl_kv8_append(jl_ctx *ctx, const jl_kv8_append_args *args, void *stream)
     if (rc) return fail(ctx, rc, "%s", message);
     if (args->tokens == 0) return JL_OK;
     DeviceGuard guard(ctx->device);
-    const cudaError_t e = kv8_append_launch(*args, ctx->sm_count, static_cast<cudaStream_t>(stream));
+    const cudaError_t e = kv8_append_launch(*args, {ctx->sm_count, ctx->use_pdl, static_cast<cudaStream_t>(stream)});
     if (e != cudaSuccess) return fail(ctx, JL_ERR_CUDA, "append launch failed: %s", cudaGetErrorString(e));
     ctx->counters.kernel_launches++;
     return JL_OK;
@@ -2332,7 +2332,7 @@ int32_t jl_kv8_attention(jl_ctx *ctx, jl_kv8_workspace *ws, const jl_kv8_attenti
     JL_REQUIRE(ctx, owns(ctx, ws), JL_ERR_INVALID, "the workspace is not one of this context's");
     if (args->rows == 0) return JL_OK;
     DeviceGuard guard(ctx->device);
-    const cudaError_t e = kv8_attention_launch(*args, ws->scratch, ctx->sm_count, static_cast<cudaStream_t>(stream));
+    const cudaError_t e = kv8_attention_launch(*args, ws->scratch, {ctx->sm_count, ctx->use_pdl, static_cast<cudaStream_t>(stream)});
     if (e != cudaSuccess) return fail(ctx, JL_ERR_CUDA, "attention launch failed: %s", cudaGetErrorString(e));
     ctx->counters.kernel_launches++;
     return JL_OK;

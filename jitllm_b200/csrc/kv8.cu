@@ -76,6 +76,8 @@ __global__ void __launch_bounds__(kMapThreads) map_kernel(const MapParams p) {
     __shared__ bool s_last;
     const jl_kv8_map_args &a = p.a;
     const int n = a.sequences, tid = threadIdx.x;
+    pdl_launch_dependents();
+    pdl_wait();
     uint32_t *token_start = smem, *block_start = smem + n;
     int32_t *kept = reinterpret_cast<int32_t *>(smem + 2 * n);  // held; below 0: the sequence is refused
     auto block_of = [&](uint32_t position) { return uint32_t((uint64_t(position) * p.divide) >> p.shift); };
@@ -197,7 +199,7 @@ __global__ void __launch_bounds__(kMapThreads) map_kernel(const MapParams p) {
 }
 
 template <int EACH>
-cudaError_t map_launch(const MapParams &p, int64_t most, int ctas, cudaStream_t stream) {
+cudaError_t map_launch(const MapParams &p, int64_t most, int ctas, const Kv8Launch &l) {
     const size_t bytes = size_t(p.a.sequences) * 12;
     if (bytes > 40 * 1024) {  // 48 KB with what the kernel has besides
         static std::atomic<uint64_t> configured{0};  // a bit for each device
@@ -205,8 +207,7 @@ cudaError_t map_launch(const MapParams &p, int64_t most, int ctas, cudaStream_t 
         if (e != cudaSuccess) return e;
     }
     const int64_t grid = (most + EACH * kMapThreads - 1) / (EACH * kMapThreads);
-    map_kernel<EACH><<<int(std::max(int64_t(1), std::min(int64_t(ctas), grid))), kMapThreads, bytes, stream>>>(p);
-    return cudaGetLastError();
+    return kv8_launch(map_kernel<EACH>, unsigned(std::max(int64_t(1), std::min(int64_t(ctas), grid))), kMapThreads, bytes, l.stream, l.programmatic, p);
 }
 
 // ---- append -------------------------------------------------------------------------------------
@@ -255,6 +256,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
     constexpr int kLanes = HD <= 64 ? 8 : HD <= 128 ? 16 : 32;  // HD / 8 of them have elements
     const jl_kv8_append_args &a = p.a;
     const int sub = threadIdx.x % kLanes;
+    pdl_launch_dependents();
+    pdl_wait();
     const uint32_t heads = a.pages.kv_heads, row = blockIdx.x * uint32_t(kAppendThreads / kLanes) + threadIdx.x / kLanes;  // rows: token, side, head
     const uint32_t t = uint32_t((uint64_t(row) * p.divide_rows) >> p.shift_rows), in_token = row - t * 2 * heads;
     const bool values = in_token >= heads;
@@ -333,13 +336,11 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
 }
 
 template <int HD>
-cudaError_t append_launch(const AppendParams &p, cudaStream_t stream) {
+cudaError_t append_launch(const AppendParams &p, const Kv8Launch &l) {
     constexpr int kLanes = HD <= 64 ? 8 : HD <= 128 ? 16 : 32;
     const int64_t rows = int64_t(p.a.tokens) * p.a.pages.kv_heads * 2;
     const unsigned grid = unsigned((rows * kLanes + kAppendThreads - 1) / kAppendThreads);
-    if (p.a.ggml_type == JL_F16) append_kernel<HD, __half><<<grid, kAppendThreads, 0, stream>>>(p);
-    else append_kernel<HD, float><<<grid, kAppendThreads, 0, stream>>>(p);
-    return cudaGetLastError();
+    return kv8_launch(p.a.ggml_type == JL_F16 ? append_kernel<HD, __half> : append_kernel<HD, float>, grid, kAppendThreads, 0, l.stream, l.programmatic, p);
 }
 
 }  // namespace
@@ -352,7 +353,7 @@ void kv8_division(int divisor, uint64_t *divide, int *shift) {
     *divide = (uint64_t(1) << *shift) / uint64_t(divisor) + 1;
 }
 
-cudaError_t kv8_map_launch(const jl_kv8_map_args &a, const Kv8Scratch &s, int sm_count, cudaStream_t stream) {
+cudaError_t kv8_map_launch(const jl_kv8_map_args &a, const Kv8Scratch &s, const Kv8Launch &l) {
     MapParams p = {};
     p.a = a;
     kv8_division(a.block_tokens, &p.divide, &p.shift);
@@ -361,20 +362,20 @@ cudaError_t kv8_map_launch(const jl_kv8_map_args &a, const Kv8Scratch &s, int sm
     p.in_place = a.lengths == a.held || a.cursor_out == a.cursor;
     p.arrivals = reinterpret_cast<unsigned *>(static_cast<char *>(s.memory) + kKv8MapCounter);
     const int64_t most = std::max(a.capacity, a.sequences);
-    return most <= int64_t(sm_count) * kMapThreads ? map_launch<1>(p, most, sm_count, stream) : map_launch<4>(p, most, 2 * sm_count, stream);
+    return most <= int64_t(l.sm_count) * kMapThreads ? map_launch<1>(p, most, l.sm_count, l) : map_launch<4>(p, most, 2 * l.sm_count, l);
 }
 
-cudaError_t kv8_append_launch(const jl_kv8_append_args &a, int, cudaStream_t stream) {
+cudaError_t kv8_append_launch(const jl_kv8_append_args &a, const Kv8Launch &l) {
     AppendParams p = {};
     p.a = a;
     kv8_division(a.pages.block_tokens, &p.divide, &p.shift);
     kv8_division(2 * a.pages.kv_heads, &p.divide_rows, &p.shift_rows);
     switch (a.pages.head_dim) {
-        case 64: return append_launch<64>(p, stream);
-        case 96: return append_launch<96>(p, stream);
-        case 128: return append_launch<128>(p, stream);
-        case 192: return append_launch<192>(p, stream);
-        default: return append_launch<256>(p, stream);
+        case 64: return append_launch<64>(p, l);
+        case 96: return append_launch<96>(p, l);
+        case 128: return append_launch<128>(p, l);
+        case 192: return append_launch<192>(p, l);
+        default: return append_launch<256>(p, l);
     }
 }
 

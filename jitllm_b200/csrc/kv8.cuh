@@ -27,9 +27,31 @@ void kv8_division(int divisor, uint64_t *divide, int *shift);
 // Lets a kernel have so many bytes of dynamic shared memory on the current device; `configured` has a bit for each device.
 cudaError_t kv8_allow_shared(const void *kernel, int bytes, std::atomic<uint64_t> &configured);
 
+// One launch; programmatic: the grid may be set up while the kernel ahead of it in the stream still runs. Each of these kernels lets
+// its successor do so as soon as it starts, and touches no memory before everything ahead of it is over (pdl_wait).
+template <typename P>
+cudaError_t kv8_launch(void (*kernel)(const P), unsigned grid, unsigned threads, size_t shared, cudaStream_t stream, bool programmatic, const P &params) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = shared;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = programmatic ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, params);
+}
+
 // Arguments that have passed the checks, on the current device.
-cudaError_t kv8_map_launch(const jl_kv8_map_args &a, const Kv8Scratch &s, int sm_count, cudaStream_t stream);
-cudaError_t kv8_append_launch(const jl_kv8_append_args &a, int sm_count, cudaStream_t stream);
-cudaError_t kv8_attention_launch(const jl_kv8_attention_args &a, const Kv8Scratch &s, int sm_count, cudaStream_t stream);
+struct Kv8Launch {
+    int sm_count;
+    bool programmatic;
+    cudaStream_t stream;
+};
+cudaError_t kv8_map_launch(const jl_kv8_map_args &a, const Kv8Scratch &s, const Kv8Launch &l);
+cudaError_t kv8_append_launch(const jl_kv8_append_args &a, const Kv8Launch &l);
+cudaError_t kv8_attention_launch(const jl_kv8_attention_args &a, const Kv8Scratch &s, const Kv8Launch &l);
 
 }  // namespace jl

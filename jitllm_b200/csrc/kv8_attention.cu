@@ -26,9 +26,8 @@ namespace jl {
 namespace {
 
 constexpr int kStep = 32;                // tokens that a warp takes at a time
-constexpr uint32_t kMinTiles = 1;        // that a piece of a unit has at least
 constexpr uint32_t kLongQuota = 8;       // tiles for each CTA from which on lines are cut without regard to units
-constexpr int kRowsPerLane = 4;
+constexpr int kRowsPerLane = 4;          // of up to 128 rows, short lines of which are cut by units
 constexpr int kMostSms = 160, kMostCtas = 4 * kMostSms;
 constexpr int kFlush = 2048;             // steps after which sums of 2^14 a token could pass 2^30
 constexpr float kHeadroom = 26.f;        // E moves on so that weights are below 2^27, and again when one would pass 2^30.5
@@ -52,11 +51,7 @@ struct Layout {
         else return r * kPitch + (c << 4);
     }
     // byte (= element) of a row that lane t's word w of keys starts at
-    __device__ static int key_element(int t, int w) {
-        if constexpr (HD == 64) return t * 16 + w * 4;
-        else if constexpr (HD == 96) return (w >> 1) * 32 + t * 8 + (w & 1) * 4;
-        else return (w >> 2) * 64 + t * 16 + (w & 3) * 4;
-    }
+    __device__ static constexpr int key_element(int t, int w) { return (w >> 1) * 32 + t * 8 + (w & 1) * 4; }
     // byte of a row that lane g's word j of values starts at
     __device__ static int value_element(int g, int j) {
         if constexpr (HD == 64) return g * 8 + j * 4;
@@ -77,7 +72,7 @@ struct Shape {
     static constexpr int kHeads = 4 * NT, kPartFloats = kHeads * (HD + 3);
     static_assert(kResident * kMostSms <= kMostCtas);
     static_assert(Layout<HD>::kStage >= kHeads * HD * 4);  // a stage also holds a warp's outputs
-    static_assert(kResident * (kBytes + 1200) <= 227 * 1024);
+    static_assert(kResident * (kBytes + NT * HD * 16 + 1024 + 640 * NT) <= 227 * 1024);
 };
 
 struct Params {
@@ -90,7 +85,7 @@ struct Params {
 };
 
 __device__ __forceinline__ void mma(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -173,8 +168,13 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
     __shared__ uint32_t warp_sums[kWarps], start_row, start_tile;
     __shared__ float s_m[kWarps][kHeads], s_e[kWarps][kHeads], s_l[kWarps][kHeads];
     __shared__ int s_last[2];
+    __shared__ uint32_t s_largest[kWarps][8 * NT];
+    __shared__ float s_scale[kHeads];
+    __shared__ uint4 s_query[NT][HD / 32][32];
     const jl_kv8_attention_args &a = p.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    pdl_launch_dependents();
+    pdl_wait();
     const int rows = a.token_count ? min(a.token_count[0], a.rows) : a.rows;
 
     // ---- what this CTA takes. Short lines: a piece of one unit, every unit cut into equal pieces of `quota` tiles at most, as
@@ -185,49 +185,56 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
     const int head0 = head_tile * kHeads, units = a.pages.kv_heads;
     uint32_t at = 0, end = 0, piece = 0, pieces = 0, in_row = 0, ctas = gridDim.x / p.head_tiles, quota = 0, more_than = 0, total = 0;
     int r = 0;
+    Row row = {};
     if (rows <= 32 * kRowsPerLane) {
-        uint32_t tiles[kRowsPerLane], mine = 0;
+        Row mine[kRowsPerLane];  // rows lane + 32 k
+        uint32_t tiles[kRowsPerLane] = {}, sum = 0;
 #pragma unroll
-        for (int k = 0; k < kRowsPerLane; ++k) {
-            const int i = lane * kRowsPerLane + k;
-            tiles[k] = i < rows ? tiles_of(row_at(a, i), kTile) : 0;
-            mine += tiles[k];
-        }
-        total = __reduce_add_sync(~0u, mine) * units;
-        if (uint32_t(rows) * units <= ctas && total < ctas * kLongQuota) {
-            quota = max(kMinTiles, (total + ctas - 1) / ctas);
-            uint32_t n[kRowsPerLane], sum;
-            for (;;) {
-                sum = 0;
-#pragma unroll
-                for (int k = 0; k < kRowsPerLane; ++k) sum += n[k] = (tiles[k] + quota - 1) / quota;
-                if (__reduce_add_sync(~0u, sum) * units <= ctas) break;
+        for (int k = 0; k < kRowsPerLane; ++k)
+            if (32 * k < rows && lane + 32 * k < rows) {
+                mine[k] = row_at(a, lane + 32 * k);
+                sum += tiles[k] = tiles_of(mine[k], kTile);
+            }
+        total = __reduce_add_sync(~0u, sum) * units;
+        const uint32_t whole_units = uint32_t(rows) * units;
+        if (whole_units <= ctas && total < ctas * kLongQuota) {
+            // a unit has half a piece more than its share on average
+            quota = total / max(1u, ctas - whole_units / 2);
+            uint32_t n[kRowsPerLane] = {}, all;
+            do {
                 quota += max(1u, quota / 8);
-            }
-            uint32_t before = sum;
+                sum = 0;
+                const float inverse = __fdividef(1.f, float(quota));
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const uint32_t o = __shfl_up_sync(~0u, before, d);
-                if (lane >= d) before += o;
-            }
-            if (cta >= __shfl_sync(~0u, before, 31) * units) return;
-            before = (before - sum) * units;
-            uint32_t found = 0, found_in = 0, found_n = 0;
+                for (int k = 0; k < kRowsPerLane; ++k)
+                    // the quotient's fraction is at least half a quota's part away from a whole number, and tiles are below 2^16
+                    if (32 * k < rows) sum += n[k] = tiles[k] ? uint32_t((float(tiles[k] - 1) + 0.5f) * inverse) + 1 : 0;
+                all = __reduce_add_sync(~0u, sum);
+            } while (all * units > ctas);
+            if (cta >= all * units) return;
+            uint32_t front = 0;  // pieces of the rows before 32 k
 #pragma unroll
-            for (int k = 0; k < kRowsPerLane; ++k) {
-                if (cta >= before && cta < before + n[k] * units) {
-                    found = lane * kRowsPerLane + k + 1;
-                    found_in = cta - before;
-                    found_n = n[k];
+            for (int k = 0; k < kRowsPerLane; ++k)
+                if (32 * k < rows && pieces == 0) {
+                    uint32_t before = n[k];
+#pragma unroll
+                    for (int d = 1; d < 32; d <<= 1) {
+                        const uint32_t o = __shfl_up_sync(~0u, before, d);
+                        if (lane >= d) before += o;
+                    }
+                    const uint32_t in_chunk = __shfl_sync(~0u, before, 31);
+                    const unsigned here = __ballot_sync(~0u, cta < (front + before) * units);  // the first of these lanes has it
+                    if (here) {
+                        const int from = __ffs(here) - 1;
+                        r = from + 32 * k;
+                        pieces = __shfl_sync(~0u, n[k], from);
+                        piece = cta - (front + __shfl_sync(~0u, before, from) - pieces) * units;
+                        row = {__shfl_sync(~0u, mine[k].first, from), __shfl_sync(~0u, mine[k].end, from), __shfl_sync(~0u, mine[k].slot, from)};
+                    }
+                    front += in_chunk;
                 }
-                before += n[k] * units;
-            }
-            const int from_lane = __ffs(__ballot_sync(~0u, found != 0)) - 1;
-            r = __shfl_sync(~0u, found, from_lane) - 1;
-            found_in = __shfl_sync(~0u, found_in, from_lane);
-            pieces = __shfl_sync(~0u, found_n, from_lane);
-            piece = found_in % pieces;
-            in_row = found_in / pieces;  // the unit, until enter() knows the row's tiles
+            in_row = piece / pieces;  // the unit
+            piece -= in_row * pieces;
         }
     }
     if (pieces == 0) {
@@ -274,12 +281,14 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
         const int32_t *line;
     } seg;
     auto enter = [&]() {
-        const Row row = row_at(a, r);
+        if (!pieces) row = row_at(a, r);
         seg.tiles = tiles_of(row, kTile);
         uint32_t unit = in_row;
         if (pieces) {
-            seg.tile = seg.tiles * piece / pieces;
-            seg.take = seg.tiles * (piece + 1) / pieces - seg.tile;
+            seg.take = seg.tiles / pieces;
+            const uint32_t longer = seg.tiles - seg.take * pieces;
+            seg.tile = piece * seg.take + min(piece, longer);
+            seg.take += piece < longer;
         } else {
             unit = in_row / seg.tiles;
             seg.tile = in_row % seg.tiles;
@@ -311,11 +320,35 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
         code_at = good ? block * a.pages.block_stride + in_block * HD : -1;
         scale_at = good ? block * a.pages.scale_stride + in_block : -1;
     };
-    auto issue = [&](int i) {
+    // Keys, scales and mask of step i, and its values, as groups of copies of their own.
+    auto copy_rows = [&](int i, const int8_t *pages, uint32_t stage) {
+        if constexpr (PAGED16) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int64_t code = __shfl_sync(~0u, code_at, 2 * (i & 15) + half);
+                if (code >= 0) {
+                    const int8_t *src = pages + code + lane * 16;
+#pragma unroll
+                    for (int n = 0; n < HD / 32; ++n) {
+                        const int piece16 = n * 32 + lane;
+                        copy16(stage + L::piece(16 * half + piece16 / (HD / 16), piece16 % (HD / 16)), src + n * 512);
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < HD / 16; ++n) {
+                const int piece16 = n * 32 + lane, row32 = piece16 / (HD / 16), c = piece16 % (HD / 16);
+                const int64_t src = __shfl_sync(~0u, code_at, row32);
+                if (src >= 0) copy16(stage + L::piece(row32, c), pages + src + c * 16);
+            }
+        }
+    };
+    auto issue_keys = [&](int i) {
         if (i < seg.mine) {
             const uint32_t stage = ring_at + uint32_t(i % S::kStages) * L::kStage, j0 = step_at(i);
             unsigned mask = (j0 < seg.first ? ~0u << (seg.first - j0) : ~0u) & (seg.to - j0 < 32 ? (1u << (seg.to - j0)) - 1 : ~0u);
-            int64_t scale = scale_at;
+            int64_t scale;
             if constexpr (PAGED16) {
                 if (i % 16 == 0) {
                     place(ahead, my_token(i));
@@ -323,35 +356,12 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
                 }
                 scale = __shfl_sync(~0u, scale_at, 2 * (i & 15) + (lane >> 4));
                 if (scale >= 0) scale += lane & 15;
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const int64_t code = __shfl_sync(~0u, code_at, 2 * (i & 15) + half);
-                    if (code >= 0) {
-                        const int8_t *k = a.pages.k + code + lane * 16, *v = a.pages.v + code + lane * 16;
-#pragma unroll
-                        for (int n = 0; n < HD / 32; ++n) {
-                            const int piece16 = n * 32 + lane;
-                            const uint32_t dst = stage + L::piece(16 * half + piece16 / (HD / 16), piece16 % (HD / 16));
-                            copy16(dst, k + n * 512);
-                            copy16(dst + L::kValues, v + n * 512);
-                        }
-                    }
-                }
             } else {
                 place(ahead, j0 + lane);
                 ahead = look_up(i + 1);
                 scale = scale_at;
-#pragma unroll
-                for (int n = 0; n < HD / 16; ++n) {
-                    const int piece16 = n * 32 + lane, row32 = piece16 / (HD / 16), c = piece16 % (HD / 16);
-                    const int64_t src = __shfl_sync(~0u, code_at, row32);
-                    const uint32_t dst = stage + L::piece(row32, c);
-                    if (src >= 0) {
-                        copy16(dst, a.pages.k + src + c * 16);
-                        copy16(dst + L::kValues, a.pages.v + src + c * 16);
-                    }
-                }
             }
+            copy_rows(i, a.pages.k, stage);
             if (scale >= 0) {
                 copy4(stage + L::kScales + 4 * lane, a.pages.k_scale + scale);
                 copy4(stage + L::kScales + 4 * kStep + 4 * lane, a.pages.v_scale + scale);
@@ -361,11 +371,18 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    auto issue_values = [&](int i) {
+        if (i < seg.mine) copy_rows(i, a.pages.v, ring_at + uint32_t(i % S::kStages) * L::kStage + L::kValues);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
     auto begin = [&]() {
         enter();
         ahead = look_up(0);
 #pragma unroll
-        for (int i = 0; i < S::kStages - 1; ++i) issue(i);
+        for (int i = 0; i < S::kStages - 1; ++i) {
+            issue_keys(i);
+            issue_values(i);
+        }
     };
 
     // Units of this CTA that others have a part of: two at most, its first and its last. Whether it was the last to arrive at one
@@ -403,24 +420,23 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
         const int mine = seg.mine, kv = seg.kv;
 
         // ---- queries: of group n, column g of the first product is byte 3 (g even) or 2 of head 4 n + g / 2, of the second byte 1 or 0.
-        // Rotated, as whole numbers below 2^30.
-        uint32_t q[NT][HD / 16][2];
-        float factor[NT];  // of head 4 n + t
-        if (mine > 0) {
+        // Rotated, as whole numbers below 2^30. A warp does its share of the words, and takes the others' from shared memory.
+        {
+            constexpr int kShare = HD / 16 / kWarps + (HD / 16 % kWarps != 0);
             const int pos = a.positions[r];
             const bool outside = a.rope_cos && pos >= a.rope_rows;
             const uint32_t select_high = g & 1 ? 0x0062 : 0x0073, select_low = g & 1 ? 0x0040 : 0x0051;
+            float x[NT][kShare][4];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const int head = head0 + 4 * n + (g >> 1);
-                float x[HD / 16][4];
                 uint32_t largest = outside ? 0x7f800000u : 0u;  // of the elements' magnitudes, as bits
                 const int64_t q_at = int64_t(r) * a.q_stride + int64_t(kv * p.group + head) * HD;
 #pragma unroll
-                for (int w = 0; w < HD / 16; ++w) {
-                    const int el = L::key_element(t, w);
+                for (int i = 0; i < kShare; ++i) {
+                    const int word = warp * kShare + i, el = L::key_element(t, word);
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (head < p.group) {
+                    if (word < HD / 16 && head < p.group && pos >= 0) {
                         if (a.ggml_type == JL_F16) {
                             const uint2 h = *reinterpret_cast<const uint2 *>(static_cast<const __half *>(a.q) + q_at + el);
                             const float2 lo = __half22float2(*reinterpret_cast<const __half2 *>(&h.x)), hi = __half22float2(*reinterpret_cast<const __half2 *>(&h.y));
@@ -428,34 +444,50 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
                         } else {
                             v = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + q_at + el);
                         }
+                        if (a.rope_cos && !outside) {
+                            const int64_t angle = int64_t(pos) * (HD / 2) + el / 2;
+                            const float2 c = *reinterpret_cast<const float2 *>(a.rope_cos + angle), s = *reinterpret_cast<const float2 *>(a.rope_sin + angle);
+                            v = make_float4(v.x * c.x - v.y * s.x, v.x * s.x + v.y * c.x, v.z * c.y - v.w * s.y, v.z * s.y + v.w * c.y);
+                        }
                     }
-                    if (a.rope_cos && !outside) {
-                        const int64_t angle = int64_t(pos) * (HD / 2) + el / 2;
-                        const float2 c = *reinterpret_cast<const float2 *>(a.rope_cos + angle), s = *reinterpret_cast<const float2 *>(a.rope_sin + angle);
-                        v = make_float4(v.x * c.x - v.y * s.x, v.x * s.x + v.y * c.x, v.z * c.y - v.w * s.y, v.z * s.y + v.w * c.y);
-                    }
-                    x[w][0] = v.x, x[w][1] = v.y, x[w][2] = v.z, x[w][3] = v.w;
+                    x[n][i][0] = v.x, x[n][i][1] = v.y, x[n][i][2] = v.z, x[n][i][3] = v.w;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) largest = max(largest, __float_as_uint(x[w][k]) & 0x7fffffffu);
+                    for (int k = 0; k < 4; ++k) largest = max(largest, __float_as_uint(x[n][i][k]) & 0x7fffffffu);
                 }
                 largest = max(largest, __shfl_xor_sync(~0u, largest, 1));
                 largest = max(largest, __shfl_xor_sync(~0u, largest, 2));
+                if (t == 0) s_largest[warp][n * 8 + g] = largest;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                uint32_t largest = 0;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) largest = max(largest, s_largest[w][n * 8 + g]);
                 const bool finite = largest < 0x7f800000u;
                 // 2^(29 - exponent of the largest), which may be 2^156, in two factors
                 const int shift = finite ? 29 - (int(largest >> 23) - 127) : 0, rest = max(shift - 126, 0);
                 const float up = __uint_as_float(uint32_t(127 + shift - rest) << 23), up_rest = __uint_as_float(uint32_t(127 + rest) << 23);
 #pragma unroll
-                for (int w = 0; w < HD / 16; ++w) {
+                for (int i = 0; i < kShare; ++i) {
+                    const int word = warp * kShare + i;
                     uint32_t b[4];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) b[k] = signed_bytes(finite ? __float2int_rn(x[w][k] * up * up_rest) : 0);
-                    q[n][w][0] = __byte_perm(__byte_perm(b[0], b[1], select_high), __byte_perm(b[2], b[3], select_high), 0x5410);
-                    q[n][w][1] = __byte_perm(__byte_perm(b[0], b[1], select_low), __byte_perm(b[2], b[3], select_low), 0x5410);
+                    for (int k = 0; k < 4; ++k) b[k] = signed_bytes(finite ? __float2int_rn(x[n][i][k] * up * up_rest) : 0);
+                    if (word < HD / 16) {
+                        uint32_t *to = reinterpret_cast<uint32_t *>(&s_query[n][word / 2][lane]) + (word & 1);
+                        to[0] = __byte_perm(__byte_perm(b[0], b[1], select_high), __byte_perm(b[2], b[3], select_high), 0x5410);
+                        to[2] = __byte_perm(__byte_perm(b[0], b[1], select_low), __byte_perm(b[2], b[3], select_low), 0x5410);
+                    }
                 }
-                // head 4 n + t is that of lanes with g = 2 t
-                factor[n] = __shfl_sync(~0u, finite ? a.scale * kLog2e * __uint_as_float(uint32_t(127 - shift + rest) << 23) * __uint_as_float(uint32_t(127 - rest) << 23) : CUDART_NAN_F, t * 8);
+                if (warp == 0 && t == 0 && (g & 1) == 0)
+                    s_scale[4 * n + g / 2] = finite ? a.scale * kLog2e * __uint_as_float(uint32_t(127 - shift + rest) << 23) * __uint_as_float(uint32_t(127 - rest) << 23) : CUDART_NAN_F;
             }
+            __syncthreads();
         }
+        float factor[NT];  // of head 4 n + t
+#pragma unroll
+        for (int n = 0; n < NT; ++n) factor[n] = s_scale[4 * n + t];
 
         // ---- one pass over this warp's tokens: lane (g, t) has tokens g, g + 8, g + 16, g + 24 of a step, heads 4 n + t, elements of
         // column g. The four tokens of g are bytes of one word of weights, and so are those of t and of t + 4 in a word of values.
@@ -491,35 +523,29 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
                     c[0][2 * k] = c[0][2 * k + 1] = c[1][2 * k] = c[1][2 * k + 1] = 0;
                 }
         };
+        // A step's keys are free when its scores are done, its values when they are added: both are refilled then, kStages steps ahead.
+        issue_keys(S::kStages - 1);
+        issue_values(S::kStages - 1);
         for (int i = 0; i < mine; ++i) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
-            __syncwarp();
-            issue(i + S::kStages - 1);
             const unsigned char *stage = ring + (i % S::kStages) * L::kStage;
-            const uint32_t stage_at = ring_at + (i % S::kStages) * L::kStage;
+            asm volatile("cp.async.wait_group %0;" ::"n"(2 * S::kStages - 1) : "memory");
+            __syncwarp();
 
             int s[NT][2][2][4] = {};  // tokens g and g + 8, g + 16 and g + 24; bytes 3 and 2, 1 and 0
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int rk = g + 16 * half;
-                constexpr int kWords = HD == 96 ? 2 : 4;
+            for (int w = 0; w < HD / 16; w += 2) {
+                uint4 q[NT];  // the first product's words w and w + 1, the second's
 #pragma unroll
-                for (int w = 0; w < HD / 16; w += kWords) {
-                    uint32_t x[kWords], y[kWords];
-                    const int el = L::key_element(t, w);
-                    if constexpr (HD == 96) {
-                        const uint2 u = lds64(stage_at + rk * L::kPitch + el), v = lds64(stage_at + (rk + 8) * L::kPitch + el);
-                        x[0] = u.x, x[1] = u.y, y[0] = v.x, y[1] = v.y;
-                    } else {
-                        const uint4 u = lds128(stage_at + L::piece(rk, el >> 4)), v = lds128(stage_at + L::piece(rk + 8, el >> 4));
-                        x[0] = u.x, x[1] = u.y, x[kWords - 2] = u.z, x[kWords - 1] = u.w, y[0] = v.x, y[1] = v.y, y[kWords - 2] = v.z, y[kWords - 1] = v.w;
+                for (int n = 0; n < NT; ++n) q[n] = s_query[n][w / 2][lane];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int rk = g + 16 * half, el = L::key_element(t, w);
+                    const uint2 x = *reinterpret_cast<const uint2 *>(stage + L::piece(rk, el >> 4) + (el & 15)), y = *reinterpret_cast<const uint2 *>(stage + L::piece(rk + 8, el >> 4) + (el & 15));
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        mma(s[n][half][0], x.x, y.x, x.y, y.y, q[n].x, q[n].y);
+                        mma(s[n][half][1], x.x, y.x, x.y, y.y, q[n].z, q[n].w);
                     }
-#pragma unroll
-                    for (int k = 0; k < kWords; k += 2)
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-#pragma unroll
-                            for (int b = 0; b < 2; ++b) mma(s[n][half][b], x[k], y[k], x[k + 1], y[k + 1], q[n][w + k][b], q[n][w + k + 1][b]);
                 }
             }
 
@@ -582,6 +608,10 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
                     }
             }
 
+            __syncwarp();  // every lane has read keys and scales
+            issue_keys(i + S::kStages);
+            asm volatile("cp.async.wait_group %0;" ::"n"(2 * S::kStages - 1) : "memory");
+            __syncwarp();
             // values: of a word of column g, elements 0 and 1 are rows g and g + 8 of one product, 2 and 3 of the next
 #pragma unroll
             for (int j0 = 0; j0 < L::kQuads; j0 += L::kLoad) {
@@ -589,12 +619,12 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
                 const int el = L::value_element(g, j0);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const uint32_t at_near = stage_at + L::kValues + L::piece(t + 8 * k, el >> 4) + (el & 15), at_far = stage_at + L::kValues + L::piece(t + 4 + 8 * k, el >> 4) + (el & 15);
+                    const unsigned char *at_near = stage + L::kValues + L::piece(t + 8 * k, el >> 4) + (el & 15), *at_far = stage + L::kValues + L::piece(t + 4 + 8 * k, el >> 4) + (el & 15);
                     if constexpr (L::kLoad == 2) {
-                        const uint2 x = lds64(at_near), y = lds64(at_far);
+                        const uint2 x = *reinterpret_cast<const uint2 *>(at_near), y = *reinterpret_cast<const uint2 *>(at_far);
                         near[0][k] = x.x, near[1][k] = x.y, far[0][k] = y.x, far[1][k] = y.y;
                     } else {
-                        near[0][k] = lds32(at_near), far[0][k] = lds32(at_far);
+                        near[0][k] = *reinterpret_cast<const uint32_t *>(at_near), far[0][k] = *reinterpret_cast<const uint32_t *>(at_far);
                     }
                 }
 #pragma unroll
@@ -611,6 +641,8 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
                         }
                 }
             }
+            __syncwarp();  // every lane has read the values
+            issue_values(i + S::kStages);
             if (++since == kFlush) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) flush(n, 1.f);
@@ -772,7 +804,7 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
 }
 
 template <int HD, int NT, bool PAGED16>
-cudaError_t launch(Params &p, const Kv8Scratch &s, int sm_count, cudaStream_t stream) {
+cudaError_t launch(Params &p, const Kv8Scratch &s, const Kv8Launch &l) {
     using S = Shape<HD, NT>;
     static std::atomic<uint64_t> configured{0};  // a bit for each device
     const cudaError_t e = kv8_allow_shared(reinterpret_cast<const void *>(attention_kernel<HD, NT, PAGED16>), S::kBytes, configured);
@@ -782,19 +814,18 @@ cudaError_t launch(Params &p, const Kv8Scratch &s, int sm_count, cudaStream_t st
     int64_t most = int64_t(a.blocks_per_slot) * a.pages.block_tokens;
     if (a.window > 0) most = std::min(most, int64_t(a.window) + 15);
     p.head_tiles = (p.group + S::kHeads - 1) / S::kHeads;
-    const int64_t tiles = (most + S::kTile - 1) / S::kTile * a.pages.kv_heads * a.rows, resident = std::max(1, sm_count * S::kResident / p.head_tiles);
+    const int64_t tiles = (most + S::kTile - 1) / S::kTile * a.pages.kv_heads * a.rows, resident = std::max(1, l.sm_count * S::kResident / p.head_tiles);
     p.arrivals = static_cast<unsigned *>(s.memory);
     p.parts = reinterpret_cast<float *>(static_cast<char *>(s.memory) + kKv8CounterBytes);
-    attention_kernel<HD, NT, PAGED16><<<int(std::min(tiles, resident)) * p.head_tiles, S::kThreads, S::kBytes, stream>>>(p);
-    return cudaGetLastError();
+    return kv8_launch(attention_kernel<HD, NT, PAGED16>, unsigned(std::min(tiles, resident)) * p.head_tiles, S::kThreads, S::kBytes, l.stream, l.programmatic, p);
 }
 
 template <int HD>
-cudaError_t launch_variant(Params &p, const Kv8Scratch &s, int sm_count, cudaStream_t stream) {
+cudaError_t launch_variant(Params &p, const Kv8Scratch &s, const Kv8Launch &l) {
     const bool paged16 = p.a.pages.block_tokens % 16 == 0;
     if constexpr (HD <= 128)
-        if (p.group > 4) return paged16 ? launch<HD, 2, true>(p, s, sm_count, stream) : launch<HD, 2, false>(p, s, sm_count, stream);
-    return paged16 ? launch<HD, 1, true>(p, s, sm_count, stream) : launch<HD, 1, false>(p, s, sm_count, stream);
+        if (p.group > 4) return paged16 ? launch<HD, 2, true>(p, s, l) : launch<HD, 2, false>(p, s, l);
+    return paged16 ? launch<HD, 1, true>(p, s, l) : launch<HD, 1, false>(p, s, l);
 }
 
 static_assert(kMostCtas * 4 <= kKv8MapCounter);
@@ -820,17 +851,17 @@ void kv8_scratch_free(Kv8Scratch *s) {
     s->memory = nullptr;
 }
 
-cudaError_t kv8_attention_launch(const jl_kv8_attention_args &a, const Kv8Scratch &s, int sm_count, cudaStream_t stream) {
+cudaError_t kv8_attention_launch(const jl_kv8_attention_args &a, const Kv8Scratch &s, const Kv8Launch &l) {
     Params p = {};
     p.a = a;
     kv8_division(a.pages.block_tokens, &p.divide, &p.shift);
     p.group = a.heads / a.pages.kv_heads;
     switch (a.pages.head_dim) {
-        case 64: return launch_variant<64>(p, s, sm_count, stream);
-        case 96: return launch_variant<96>(p, s, sm_count, stream);
-        case 128: return launch_variant<128>(p, s, sm_count, stream);
-        case 192: return launch_variant<192>(p, s, sm_count, stream);
-        default: return launch_variant<256>(p, s, sm_count, stream);
+        case 64: return launch_variant<64>(p, s, l);
+        case 96: return launch_variant<96>(p, s, l);
+        case 128: return launch_variant<128>(p, s, l);
+        case 192: return launch_variant<192>(p, s, l);
+        default: return launch_variant<256>(p, s, l);
     }
 }
 
