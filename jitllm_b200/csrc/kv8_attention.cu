@@ -66,13 +66,14 @@ template <int HD, int NT>
 struct Shape {
     static constexpr int kWarps = HD <= 128 ? 4 : 2, kThreads = 32 * kWarps;
     static constexpr int kTile = kStep * kWarps;  // tokens of a tile
-    static constexpr int kResident = HD == 64 ? (NT == 1 ? 4 : 3) : HD == 96 ? (NT == 1 ? 4 : 3) : HD == 128 ? (NT == 1 ? 3 : 2) : 3;  // CTAs per SM
     static constexpr int kStages = HD == 64 ? (NT == 1 ? 3 : 4) : HD == 128 && NT == 2 ? 3 : 2;
     static constexpr int kRing = kStages * Layout<HD>::kStage, kBytes = kWarps * kRing;
     static constexpr int kHeads = 4 * NT, kPartFloats = kHeads * (HD + 3);
+    static constexpr int kShare = HD / 16 / kWarps + (HD / 16 % kWarps != 0);  // words of the queries that a warp prepares
+    static constexpr int kResident = HD <= 96 ? (NT == 1 ? 4 : 3) : HD == 128 ? (NT == 1 ? 3 : 2) : 3;  // CTAs per SM
     static_assert(kResident * kMostSms <= kMostCtas);
     static_assert(Layout<HD>::kStage >= kHeads * HD * 4);  // a stage also holds a warp's outputs
-    static_assert(kResident * (kBytes + NT * HD * 16 + 1024 + 640 * NT) <= 227 * 1024);
+    static_assert(kResident * (kBytes + NT * HD * 16 + kWarps * kShare * (NT * 256 + 64) + 128 * kHeads + 1024) <= 228 * 1024);
 };
 
 struct Params {
@@ -114,6 +115,11 @@ __device__ __forceinline__ float step_down(float from, float to) {
 }
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// SIZE bytes, or as many zeros
+template <int SIZE>
+__device__ __forceinline__ void copy_or_zero(uint32_t dst, const void *src, bool copy) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(SIZE), "r"(copy ? SIZE : 0) : "memory");
 }
 __device__ __forceinline__ void copy4(uint32_t dst, const void *src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
@@ -171,9 +177,10 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
     __shared__ uint32_t s_largest[kWarps][8 * NT];
     __shared__ float s_scale[kHeads];
     __shared__ uint4 s_query[NT][HD / 32][32];
+    constexpr int kShare = S::kShare;
+    __shared__ float4 s_raw[kWarps][kShare][NT][16], s_turn[kWarps][kShare][4];
     const jl_kv8_attention_args &a = p.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    pdl_launch_dependents();
     pdl_wait();
     const int rows = a.token_count ? min(a.token_count[0], a.rows) : a.rows;
 
@@ -277,7 +284,7 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
     // token from + (warp + warps i) 32.
     struct Segment {
         uint32_t first, from, to, tiles, tile, take;
-        int kv, mine;
+        int kv, mine, pos;
         const int32_t *line;
     } seg;
     auto enter = [&]() {
@@ -300,6 +307,7 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
         seg.to = min(row.end, seg.from + seg.take * kTile);
         const int steps = seg.to > seg.from ? int((seg.to - seg.from + kStep - 1) / kStep) : 0;
         seg.mine = steps > warp ? (steps - warp + kWarps - 1) / kWarps : 0;
+        seg.pos = a.positions[r];
         seg.line = a.block_table + int64_t(row.slot) * a.blocks_per_slot;
     };
     auto step_at = [&](int i) { return seg.from + uint32_t(warp + i * kWarps) * kStep; };
@@ -375,9 +383,35 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
         if (i < seg.mine) copy_rows(i, a.pages.v, ring_at + uint32_t(i % S::kStages) * L::kStage + L::kValues);
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    // Queries of a segment, as they are, and their places in the rotation tables: the words that this warp prepares. On the way before the keys.
+    auto load_queries = [&]() {
+#pragma unroll
+        for (int i = 0; i < kShare; ++i) {
+            const int word = warp * kShare + i, el = L::key_element(t, word);
+            if (word >= HD / 16) continue;
+            if ((g & 1) == 0)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const int head = head0 + 4 * n + (g >> 1);
+                    const bool here = head < p.group;
+                    const int64_t at_q = here ? int64_t(r) * a.q_stride + int64_t(seg.kv * p.group + head) * HD + el : 0;
+                    const uint32_t dst = smem_u32(&s_raw[warp][i][n][(g >> 1) * 4 + t]);
+                    if (a.ggml_type == JL_F16) copy_or_zero<8>(dst, static_cast<const __half *>(a.q) + at_q, here);
+                    else copy_or_zero<16>(dst, static_cast<const float *>(a.q) + at_q, here);
+                }
+            else if (g == 1 && a.rope_cos && seg.pos >= 0 && seg.pos < a.rope_rows) {
+                const int64_t angle = int64_t(seg.pos) * (HD / 2) + el / 2;
+                const uint32_t dst = smem_u32(&s_turn[warp][i][t]);
+                copy_or_zero<8>(dst, a.rope_cos + angle, true);
+                copy_or_zero<8>(dst + 8, a.rope_sin + angle, true);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
     auto begin = [&]() {
         enter();
         ahead = look_up(0);
+        load_queries();
 #pragma unroll
         for (int i = 0; i < S::kStages - 1; ++i) {
             issue_keys(i);
@@ -422,32 +456,26 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
         // ---- queries: of group n, column g of the first product is byte 3 (g even) or 2 of head 4 n + g / 2, of the second byte 1 or 0.
         // Rotated, as whole numbers below 2^30. A warp does its share of the words, and takes the others' from shared memory.
         {
-            constexpr int kShare = HD / 16 / kWarps + (HD / 16 % kWarps != 0);
-            const int pos = a.positions[r];
-            const bool outside = a.rope_cos && pos >= a.rope_rows;
+            const bool outside = a.rope_cos && seg.pos >= a.rope_rows, turn = a.rope_cos && seg.pos >= 0 && !outside;
             const uint32_t select_high = g & 1 ? 0x0062 : 0x0073, select_low = g & 1 ? 0x0040 : 0x0051;
             float x[NT][kShare][4];
+            asm volatile("cp.async.wait_group %0;" ::"n"(2 * S::kStages - 2) : "memory");
+            __syncwarp();
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const int head = head0 + 4 * n + (g >> 1);
                 uint32_t largest = outside ? 0x7f800000u : 0u;  // of the elements' magnitudes, as bits
-                const int64_t q_at = int64_t(r) * a.q_stride + int64_t(kv * p.group + head) * HD;
 #pragma unroll
                 for (int i = 0; i < kShare; ++i) {
-                    const int word = warp * kShare + i, el = L::key_element(t, word);
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (word < HD / 16 && head < p.group && pos >= 0) {
+                    if (warp * kShare + i < HD / 16) {
+                        v = s_raw[warp][i][n][(g >> 1) * 4 + t];
                         if (a.ggml_type == JL_F16) {
-                            const uint2 h = *reinterpret_cast<const uint2 *>(static_cast<const __half *>(a.q) + q_at + el);
-                            const float2 lo = __half22float2(*reinterpret_cast<const __half2 *>(&h.x)), hi = __half22float2(*reinterpret_cast<const __half2 *>(&h.y));
+                            const float2 lo = __half22float2(*reinterpret_cast<const __half2 *>(&v.x)), hi = __half22float2(*reinterpret_cast<const __half2 *>(&v.y));
                             v = make_float4(lo.x, lo.y, hi.x, hi.y);
-                        } else {
-                            v = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + q_at + el);
                         }
-                        if (a.rope_cos && !outside) {
-                            const int64_t angle = int64_t(pos) * (HD / 2) + el / 2;
-                            const float2 c = *reinterpret_cast<const float2 *>(a.rope_cos + angle), s = *reinterpret_cast<const float2 *>(a.rope_sin + angle);
-                            v = make_float4(v.x * c.x - v.y * s.x, v.x * s.x + v.y * c.x, v.z * c.y - v.w * s.y, v.z * s.y + v.w * c.y);
+                        if (turn) {
+                            const float4 c = s_turn[warp][i][t];  // two cosines, two sines
+                            v = make_float4(v.x * c.x - v.y * c.z, v.x * c.z + v.y * c.x, v.z * c.y - v.w * c.w, v.z * c.w + v.w * c.y);
                         }
                     }
                     x[n][i][0] = v.x, x[n][i][1] = v.y, x[n][i][2] = v.z, x[n][i][3] = v.w;
@@ -669,6 +697,7 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
         in_row += seg.take;
         if (in_row == seg.tiles * uint32_t(units)) ++r, in_row = 0;
         const bool more = !pieces && at < end;
+        if (!more) pdl_launch_dependents();  // not before: early CTAs of the next launch would take the places that spread this one's out
         if (more) begin();
         float4 *out_w = reinterpret_cast<float4 *>(ring + (S::kStages - 1) * L::kStage);
 #pragma unroll
@@ -755,18 +784,22 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w][my_head]), etop = fmaxf(etop, s_e[w][my_head]);
-        float *keep = reinterpret_cast<float *>(smem);  // [part][head]
 #pragma unroll 4
         for (int k = tid / kHeads; k < n; k += kThreads / kHeads) {
             const float *stats = part_of(k) + kHeads * HD + my_head;
             sum += __ldcg(stats + 2 * kHeads) * step_down(__ldcg(stats), top);
-            keep[k * kHeads + my_head] = step_down(__ldcg(stats + kHeads), etop);
         }
 #pragma unroll
         for (int d = kHeads; d < 32; d <<= 1) sum += __shfl_xor_sync(~0u, sum, d);
         if (lane < kHeads) s_l[warp][lane] = sum;
-        __syncthreads();
-        // outputs: a warp has every fourth part
+        float head_etop[NT];  // of head 4 n + t
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            head_etop[n] = -CUDART_INF_F;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) head_etop[n] = fmaxf(head_etop[n], s_e[w][4 * n + t]);
+        }
+        // outputs: parts are dealt out to the warps
         constexpr int kUnroll = NT * L::kQuads <= 4 ? 4 : NT * L::kQuads <= 8 ? 2 : 1;
         float4 x[NT * L::kQuads];
 #pragma unroll
@@ -777,27 +810,26 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
 #pragma unroll
             for (int f = 0; f < NT * L::kQuads; ++f) {
                 const float4 y = __ldcg(src + f * 32);
-                const float w = keep[k * kHeads + 4 * (f / L::kQuads) + t];
+                const float w = step_down(__ldcg(part_of(k) + kHeads * HD + kHeads + 4 * (f / L::kQuads) + t), head_etop[f / L::kQuads]);
                 x[f].x += y.x * w, x[f].y += y.y * w, x[f].z += y.z * w, x[f].w += y.w * w;
             }
         }
-        float4 *warp_out = reinterpret_cast<float4 *>(smem + kMostCtas * kHeads * 4);  // behind `keep`
-        static_assert(kMostCtas * kHeads * 4 + kWarps * NT * HD * 16 <= S::kBytes);
+        float4 *warp_out = reinterpret_cast<float4 *>(smem);
 #pragma unroll
         for (int f = 0; f < NT * L::kQuads; ++f) warp_out[(warp * NT * L::kQuads + f) * 32 + lane] = x[f];
         __syncthreads();
         for (int f = warp; f < NT * L::kQuads; f += kWarps) {
             const int head = 4 * (f / L::kQuads) + t;
             float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-            float all = 0.f, head_top = -CUDART_INF_F, head_etop = -CUDART_INF_F;
+            float all = 0.f, all_top = -CUDART_INF_F, all_etop = -CUDART_INF_F;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
                 const float4 z = warp_out[(w * NT * L::kQuads + f) * 32 + lane];
                 y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
                 all += s_l[w][head];
-                head_top = fmaxf(head_top, s_m[w][head]), head_etop = fmaxf(head_etop, s_e[w][head]);
+                all_top = fmaxf(all_top, s_m[w][head]), all_etop = fmaxf(all_etop, s_e[w][head]);
             }
-            finish(f, unit.r, unit.kv, y, head_top, head_etop, all);
+            finish(f, unit.r, unit.kv, y, all_top, all_etop, all);
         }
         __syncthreads();
     }
@@ -821,7 +853,7 @@ cudaError_t launch(Params &p, const Kv8Scratch &s, const Kv8Launch &l) {
 }
 
 template <int HD>
-cudaError_t launch_variant(Params &p, const Kv8Scratch &s, const Kv8Launch &l) {
+cudaError_t launch_head(Params &p, const Kv8Scratch &s, const Kv8Launch &l) {
     const bool paged16 = p.a.pages.block_tokens % 16 == 0;
     if constexpr (HD <= 128)
         if (p.group > 4) return paged16 ? launch<HD, 2, true>(p, s, l) : launch<HD, 2, false>(p, s, l);
@@ -857,11 +889,11 @@ cudaError_t kv8_attention_launch(const jl_kv8_attention_args &a, const Kv8Scratc
     kv8_division(a.pages.block_tokens, &p.divide, &p.shift);
     p.group = a.heads / a.pages.kv_heads;
     switch (a.pages.head_dim) {
-        case 64: return launch_variant<64>(p, s, l);
-        case 96: return launch_variant<96>(p, s, l);
-        case 128: return launch_variant<128>(p, s, l);
-        case 192: return launch_variant<192>(p, s, l);
-        default: return launch_variant<256>(p, s, l);
+        case 64: return launch_head<64>(p, s, l);
+        case 96: return launch_head<96>(p, s, l);
+        case 128: return launch_head<128>(p, s, l);
+        case 192: return launch_head<192>(p, s, l);
+        default: return launch_head<256>(p, s, l);
     }
 }
 

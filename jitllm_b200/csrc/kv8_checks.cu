@@ -92,8 +92,8 @@ int kv8_check_attention(const jl_kv8_attention_args *a, char *message, size_t n)
     KV8_REQUIRE(a, JL_ERR_INVALID, "args must not be NULL");
     int rc = check_pages(a->pages, message, n);
     if (rc) return rc;
-    KV8_REQUIRE(a->rows >= 0 && a->rows <= 1 << 20 && a->slots > 0 && a->blocks_per_slot > 0 && a->window >= 0, JL_ERR_INVALID,
-                "rows must be in 0..2^20, slots and blocks_per_slot positive, window not negative, got %d, %d, %d and %d", a->rows, a->slots,
+    KV8_REQUIRE(a->rows >= 0 && a->rows <= 1 << 16 && a->slots > 0 && a->blocks_per_slot > 0 && a->window >= 0, JL_ERR_INVALID,
+                "rows must be in 0..2^16, slots and blocks_per_slot positive, window not negative, got %d, %d, %d and %d", a->rows, a->slots,
                 a->blocks_per_slot, a->window);
     KV8_REQUIRE(a->heads > 0 && a->heads % a->pages.kv_heads == 0 && a->heads <= 16384, JL_ERR_INVALID,
                 "heads must be a multiple of kv_heads and at most 16384, got %d and %d", a->heads, a->pages.kv_heads);
