@@ -29,6 +29,9 @@ constexpr int kStep = 32;                // tokens that a warp takes at a time
 constexpr uint32_t kLongQuota = 8;       // tiles for each CTA from which on lines are cut without regard to units
 constexpr int kRowsPerLane = 4;          // of up to 128 rows, short lines of which are cut by units
 constexpr int kMostSms = 160, kMostCtas = 4 * kMostSms;
+constexpr uint32_t kGroup = 32;          // parts that are joined at once
+constexpr int kSlots = 4;                // for parts, of a CTA
+static_assert(kMostCtas <= int(kGroup * kGroup));
 constexpr int kFlush = 2048;             // steps after which sums of 2^14 a token could pass 2^30
 constexpr float kHeadroom = 26.f;        // E moves on so that weights are below 2^27, and again when one would pass 2^30.5
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
@@ -81,8 +84,8 @@ struct Params {
     uint64_t divide;   // j / block_tokens = j * divide >> shift for j < 2^31
     int shift;
     int group, head_tiles;         // query heads per KV head, units that these are
-    unsigned *arrivals;            // [CTAs], zero between launches
-    float *parts;                  // [2 * CTAs][part floats]
+    unsigned *arrivals;            // [3][CTAs], zero between launches
+    float *parts;                  // [kSlots * CTAs][part floats]
 };
 
 __device__ __forceinline__ void mma(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -173,7 +176,7 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ uint32_t warp_sums[kWarps], start_row, start_tile;
     __shared__ float s_m[kWarps][kHeads], s_e[kWarps][kHeads], s_l[kWarps][kHeads];
-    __shared__ int s_last[2];
+    __shared__ int s_last;
     __shared__ uint32_t s_largest[kWarps][8 * NT];
     __shared__ float s_scale[kHeads];
     __shared__ uint4 s_query[NT][HD / 32][32];
@@ -427,6 +430,20 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
     } shared[2];
     int n_shared = 0;
     bool arrived_last[2] = {false, false};  // thread 0
+    // A CTA's slots: the part of its first segment, of its last, and joined parts of a group that begins behind or with a unit's first CTA.
+    auto slot_of = [&](uint32_t owner, int slot) { return p.parts + ((size_t(owner) * p.head_tiles + head_tile) * kSlots + slot) * S::kPartFloats; };
+    // Thread 0: whether this CTA is the last of its unit, or, of a unit of more than kGroup parts, of its group. The last one to come sets
+    // the counter back to zero. Counters: by a unit's first CTA, by a later group's first CTA, and of the groups by the unit's first CTA.
+    auto count_in = [&](int which, uint32_t owner, uint32_t all) {
+        __threadfence();
+        const bool is_last = atomicInc(p.arrivals + which * kMostCtas + owner * p.head_tiles + head_tile, all - 1) == all - 1;
+        __threadfence();
+        return is_last;
+    };
+    auto arrive = [&](const Shared &unit) {
+        const uint32_t group = (cta - unit.first) / kGroup, in_front = group * kGroup;
+        return count_in(group > 0, unit.first + in_front, unit.parts > kGroup ? min(kGroup, unit.parts - in_front) : unit.parts);
+    };
 
     // quad f = n kQuads + j of lane (g, t): four elements of head 4 n + t
     auto finish = [&](int f, int row, int kv, float4 x, float top, float etop, float sum) {
@@ -710,7 +727,7 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
         }
         __syncthreads();
         const bool whole = first_cta == last_cta;
-        float *part = p.parts + (size_t(blockIdx.x) * 2 + (cta == first_cta)) * S::kPartFloats;
+        float *part = slot_of(cta, cta == first_cta);
         for (int f = warp; f < NT * L::kQuads; f += kWarps) {
             const int head = 4 * (f / L::kQuads) + t;
             float top = -CUDART_INF_F, etop = -CUDART_INF_F, sum = 0.f;
@@ -736,14 +753,12 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
         }
         __syncthreads();  // the part is written, the fold's stage is free
         if (!whole) {
-            const unsigned others = last_cta - first_cta;
+            const Shared unit = {row, kv, first_cta, last_cta - first_cta + 1};
             if (tid == 0) {
-                __threadfence();
-                const bool is_last = atomicInc(p.arrivals + first_cta * p.head_tiles + head_tile, others) == others;  // the last one to come sets it back to zero
+                const bool is_last = arrive(unit);
                 if (n_shared == 0) arrived_last[0] = is_last;
                 else arrived_last[1] = is_last;
             }
-            const Shared unit = {row, kv, first_cta, others + 1};
             if (n_shared == 0) shared[0] = unit;
             else shared[1] = unit;
             ++n_shared;
@@ -751,87 +766,92 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
         if (!more) break;
     }
 
-    // ---- join the units that this CTA came last to
-    if (n_shared == 0) return;
-    if (tid == 0) {
-        s_last[0] = arrived_last[0];
-        s_last[1] = arrived_last[1];
-        __threadfence();
-    }
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        if (u >= n_shared || !s_last[u]) continue;
-        const Shared &unit = shared[u];
-        const int n = int(unit.parts);
-        auto part_of = [&](int k) { return p.parts + (size_t((unit.first + k) * p.head_tiles + head_tile) * 2 + (k == 0)) * S::kPartFloats; };
-        // maxima and sums: thread i has head i mod heads of every (threads / heads)-th part
-        const int my_head = tid % kHeads;
-        float top = -CUDART_INF_F, etop = -CUDART_INF_F, sum = 0.f;
-#pragma unroll 4
-        for (int k = tid / kHeads; k < n; k += kThreads / kHeads) {
-            const float *stats = part_of(k) + kHeads * HD + my_head;
-            top = fmaxf(top, __ldcg(stats));
-            etop = fmaxf(etop, __ldcg(stats + kHeads));
-        }
-#pragma unroll
-        for (int d = kHeads; d < 32; d <<= 1) {
-            top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-            etop = fmaxf(etop, __shfl_xor_sync(~0u, etop, d));
-        }
-        __syncthreads();  // what was kept here before has been read
-        if (lane < kHeads) s_m[warp][lane] = top, s_e[warp][lane] = etop;
+    // ---- join the units that this CTA came last to: a group's parts, 32 at most, then the groups. Every warp works out the parts' weights for
+    // itself (lane (g, t) those of parts g, g + 8, ... of heads 4 n + t) and has its own quads of the outputs, so nothing is waited for in between.
+    for (int u = 0; u < n_shared; ++u) {
+        const Shared unit = u ? shared[1] : shared[0];
+        if (tid == 0) s_last = u ? arrived_last[1] : arrived_last[0];
         __syncthreads();
+        bool here = s_last;
+        const uint32_t group = (cta - unit.first) / kGroup, in_front = group * kGroup;
+        for (int level = unit.parts > kGroup ? 0 : 1; here; ++level) {
+            const bool groups = unit.parts > kGroup && level == 1;
+            const int n = level == 0 ? min(kGroup, unit.parts - in_front) : groups ? (unit.parts + kGroup - 1) / kGroup : unit.parts;
+            // part k, and its slot: that of the unit's first part is another one
+            const float *base = slot_of(unit.first + (level == 0 ? in_front : 0), groups ? 2 : 0);
+            const size_t stride = size_t(p.head_tiles) * kSlots * S::kPartFloats * (groups ? kGroup : 1);
+            const int first_slot = groups ? S::kPartFloats : level == 0 && group ? 0 : S::kPartFloats;
+            auto part_of = [&](int k) { return base + k * stride + (k ? 0 : first_slot); };
+            // sixteen parts' quads at once
+            float4 y[16];
+            auto load = [&](int f, int k0) {
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w][my_head]), etop = fmaxf(etop, s_e[w][my_head]);
-#pragma unroll 4
-        for (int k = tid / kHeads; k < n; k += kThreads / kHeads) {
-            const float *stats = part_of(k) + kHeads * HD + my_head;
-            sum += __ldcg(stats + 2 * kHeads) * step_down(__ldcg(stats), top);
-        }
+                for (int k = 0; k < 16; ++k)
+                    if (k0 + k < n) y[k] = __ldcg(reinterpret_cast<const float4 *>(part_of(k0 + k)) + f * 32 + lane);
+            };
+            if (warp < L::kQuads) load(warp, 0);
+            float top[NT], etop[NT], sum[NT], keep[NT][kGroup / 8];
 #pragma unroll
-        for (int d = kHeads; d < 32; d <<= 1) sum += __shfl_xor_sync(~0u, sum, d);
-        if (lane < kHeads) s_l[warp][lane] = sum;
-        float head_etop[NT];  // of head 4 n + t
+            for (int i = 0; i < NT; ++i) {
+                float m[kGroup / 8], e[kGroup / 8], l[kGroup / 8];
+                top[i] = etop[i] = -CUDART_INF_F;
+                sum[i] = 0.f;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            head_etop[n] = -CUDART_INF_F;
+                for (int k = 0; k < int(kGroup / 8); ++k) {
+                    m[k] = e[k] = -CUDART_INF_F;
+                    l[k] = 0.f;
+                    if (g + 8 * k < n) {
+                        const float *stats = part_of(g + 8 * k) + kHeads * HD + 4 * i + t;
+                        m[k] = __ldcg(stats), e[k] = __ldcg(stats + kHeads), l[k] = __ldcg(stats + 2 * kHeads);
+                    }
+                    top[i] = fmaxf(top[i], m[k]), etop[i] = fmaxf(etop[i], e[k]);
+                }
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) head_etop[n] = fmaxf(head_etop[n], s_e[w][4 * n + t]);
-        }
-        // outputs: parts are dealt out to the warps
-        constexpr int kUnroll = NT * L::kQuads <= 4 ? 4 : NT * L::kQuads <= 8 ? 2 : 1;
-        float4 x[NT * L::kQuads];
+                for (int d = 4; d < 32; d <<= 1) {
+                    top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], d));
+                    etop[i] = fmaxf(etop[i], __shfl_xor_sync(~0u, etop[i], d));
+                }
 #pragma unroll
-        for (int f = 0; f < NT * L::kQuads; ++f) x[f] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll kUnroll
-        for (int k = warp; k < n; k += kWarps) {
-            const float4 *src = reinterpret_cast<const float4 *>(part_of(k)) + lane;
+                for (int k = 0; k < int(kGroup / 8); ++k) {
+                    sum[i] += l[k] * step_down(m[k], top[i]);
+                    keep[i][k] = step_down(e[k], etop[i]);
+                }
 #pragma unroll
-            for (int f = 0; f < NT * L::kQuads; ++f) {
-                const float4 y = __ldcg(src + f * 32);
-                const float w = step_down(__ldcg(part_of(k) + kHeads * HD + kHeads + 4 * (f / L::kQuads) + t), head_etop[f / L::kQuads]);
-                x[f].x += y.x * w, x[f].y += y.y * w, x[f].z += y.z * w, x[f].w += y.w * w;
+                for (int d = 4; d < 32; d <<= 1) sum[i] += __shfl_xor_sync(~0u, sum[i], d);
             }
-        }
-        float4 *warp_out = reinterpret_cast<float4 *>(smem);
 #pragma unroll
-        for (int f = 0; f < NT * L::kQuads; ++f) warp_out[(warp * NT * L::kQuads + f) * 32 + lane] = x[f];
-        __syncthreads();
-        for (int f = warp; f < NT * L::kQuads; f += kWarps) {
-            const int head = 4 * (f / L::kQuads) + t;
-            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-            float all = 0.f, all_top = -CUDART_INF_F, all_etop = -CUDART_INF_F;
+            for (int i = 0; i < NT; ++i)
+                for (int j = warp; j < L::kQuads; j += kWarps) {
+                    const int f = i * L::kQuads + j;
+                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float4 z = warp_out[(w * NT * L::kQuads + f) * 32 + lane];
-                y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
-                all += s_l[w][head];
-                all_top = fmaxf(all_top, s_m[w][head]), all_etop = fmaxf(all_etop, s_e[w][head]);
-            }
-            finish(f, unit.r, unit.kv, y, all_top, all_etop, all);
+                    for (int half = 0; half < int(kGroup / 16); ++half) {
+                        if (16 * half >= n) break;
+                        if (f != warp || half) load(f, 16 * half);
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            const float w = __shfl_sync(~0u, keep[i][2 * half + k / 8], 4 * (k & 7) + t);
+                            if (16 * half + k < n) x.x += y[k].x * w, x.y += y[k].y * w, x.z += y[k].z * w, x.w += y[k].w * w;
+                        }
+                    }
+                    if (level == 1) {
+                        finish(f, unit.r, unit.kv, x, top[i], etop[i], sum[i]);
+                    } else {
+                        float *to = slot_of(unit.first + in_front, group ? 2 : 3);
+                        reinterpret_cast<float4 *>(to)[f * 32 + lane] = x;
+                        if (j == 0 && g == 0) {
+                            float *stats = to + kHeads * HD + 4 * i + t;
+                            stats[0] = top[i], stats[kHeads] = etop[i], stats[2 * kHeads] = sum[i];
+                        }
+                    }
+                }
+            if (level == 1) break;
+            __syncthreads();
+            if (tid == 0) s_last = count_in(2, unit.first, (unit.parts + kGroup - 1) / kGroup);
+            __syncthreads();
+            here = s_last;
         }
-        __syncthreads();
+        __syncthreads();  // s_last has been read
     }
 }
 
@@ -860,16 +880,16 @@ cudaError_t launch_head(Params &p, const Kv8Scratch &s, const Kv8Launch &l) {
     return paged16 ? launch<HD, 1, true>(p, s, l) : launch<HD, 1, false>(p, s, l);
 }
 
-static_assert(kMostCtas * 4 <= kKv8MapCounter);
+static_assert(3 * kMostCtas * 4 <= kKv8MapCounter);
 
 template <int HD, int NT>
-constexpr size_t kPartsPerSm = size_t(2) * Shape<HD, NT>::kResident *Shape<HD, NT>::kPartFloats * sizeof(float);
+constexpr size_t kPartsPerSm = size_t(kSlots) * Shape<HD, NT>::kResident *Shape<HD, NT>::kPartFloats * sizeof(float);
 
 }  // namespace
 
 cudaError_t kv8_scratch_create(Kv8Scratch *s, int sm_count) {
     if (sm_count > kMostSms) return cudaErrorInvalidValue;  // more CTAs than there are counters, or than a join has room for
-    // two parts for each CTA of the largest grid, of the largest kind
+    // for the CTAs of the largest grid, of the largest kind
     const size_t parts = std::max({kPartsPerSm<64, 1>, kPartsPerSm<64, 2>, kPartsPerSm<96, 1>, kPartsPerSm<96, 2>, kPartsPerSm<128, 1>, kPartsPerSm<128, 2>, kPartsPerSm<192, 1>,
                                    kPartsPerSm<256, 1>});
     cudaError_t e = cudaMalloc(&s->memory, kKv8CounterBytes + size_t(sm_count) * parts);
