@@ -64,16 +64,19 @@ struct Layout {
     }
 };
 
-// NT groups of four query heads have HD / 2 * NT accumulators; what these and the stages leave room for:
+// NT groups of four query heads have HD / 2 * NT accumulators. What these and the stages leave room for, with both sides measured (us):
+// head size 128, 2 CTAs of 3 stages and 3 CTAs of 2: 13.3 / 14.9 (32 rows at 512 of 8 KV heads), 18.0 / 20.6 (1 row at 20000); 64 with one group,
+// 4 CTAs of 3 and 3 of 4: 20.5 / 24.4 (64 rows, a window of 1000), 9.1 / 9.3 (1 row at 4000), with two groups, 2 of 6 and 3 of 4: 12.5 / 16.4 (8
+// rows at 2000 of 4 KV heads); 96, 3 of 2 and 2 of 4: 17.2 / 18.3 (16 rows at 2000), two groups 17.0 / 13.6; 256, 2 of 3 and 3 of 2: 19.0 / 20.5.
 template <int HD, int NT>
 struct Shape {
     static constexpr int kWarps = HD <= 128 ? 4 : 2, kThreads = 32 * kWarps;
     static constexpr int kTile = kStep * kWarps;  // tokens of a tile
-    static constexpr int kStages = HD == 64 ? (NT == 1 ? 3 : 4) : HD == 128 && NT == 2 ? 3 : 2;
+    static constexpr int kStages = HD == 64 ? (NT == 1 ? 3 : 6) : HD == 96 ? (NT == 1 ? 2 : 4) : 3;
     static constexpr int kRing = kStages * Layout<HD>::kStage, kBytes = kWarps * kRing;
     static constexpr int kHeads = 4 * NT, kPartFloats = kHeads * (HD + 3);
     static constexpr int kShare = HD / 16 / kWarps + (HD / 16 % kWarps != 0);  // words of the queries that a warp prepares
-    static constexpr int kResident = HD <= 96 ? (NT == 1 ? 4 : 3) : HD == 128 ? (NT == 1 ? 3 : 2) : 3;  // CTAs per SM
+    static constexpr int kResident = NT == 1 && HD == 64 ? 4 : NT == 1 && HD == 96 ? 3 : 2;  // CTAs per SM
     static_assert(kResident * kMostSms <= kMostCtas);
     static_assert(Layout<HD>::kStage >= kHeads * HD * 4);  // a stage also holds a warp's outputs
     static_assert(kResident * (kBytes + NT * HD * 16 + kWarps * kShare * (NT * 256 + 64) + 128 * kHeads + 1024) <= 228 * 1024);
