@@ -70,13 +70,13 @@ class _Call:
         self._ref = C.byref(args)
 
     def launch(self, stream: Optional[int] = None) -> None:
-        dev = self.dev
+        dev, ws = self.dev, self.workspace
+        h = dev._h
+        if h is None or (ws is not None and (ws._h is None or ws.dev._h is None)):
+            raise IllegalStateError("GPUL-LIFE-001: the device context or the workspace is closed")
         if stream is None:
-            stream = dev._lib.jl_stream(dev.handle)
-        if self.workspace is None:
-            rc = self._entry(dev.handle, self._ref, stream)
-        else:
-            rc = self._entry(dev.handle, self.workspace.handle, self._ref, stream)
+            stream = dev._lib.jl_stream(h)
+        rc = self._entry(h, self._ref, stream) if ws is None else self._entry(h, ws._h, self._ref, stream)
         if rc != 0:
             dev._check(rc)
 

@@ -353,7 +353,7 @@ class _Attention:
                 x = self.lse[r].cpu().numpy().astype(np.float64)
                 assert np.array_equal(np.isnan(x), np.isnan(lse[r])) and np.array_equal(np.isinf(x), np.isinf(lse[r]))
                 ok = np.isfinite(lse[r])
-                assert (np.abs(x - lse[r])[ok] <= ref.score_tolerance(self.d, most[r]) + 2.0 ** -23 * np.abs(lse[r][ok])).all()
+                assert (np.abs(x[ok] - lse[r][ok]) <= ref.score_tolerance(self.d, most[r]) + 2.0 ** -23 * np.abs(lse[r][ok])).all()
 
 
 LENGTHS = [0, 1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 100, 127, 128, 129, 255, 257, 300]
@@ -530,7 +530,103 @@ def test_attention_in_pages_beyond_32_bits(dev, ws):
     assert np.linalg.norm(out.cpu().numpy() - want) <= 2 * ref.score_tolerance(d, most[0]) * np.linalg.norm(want)
 
 
+def test_attention_of_a_long_sequence_of_repeated_blocks(dev, ws):
+    """More steps for a warp than its integer sums hold at once (2^16 tokens): the blocks of a row repeat, so that the output is that of
+    one round of them, and its lse that and the logarithm of the rounds."""
+    rows, heads, d, block, rounds = 64, 8, 64, 16, 5000
+    p = _Pages(dev, 4, block, heads, d, seed=3)
+    rng = np.random.default_rng(3)
+    q = rng.standard_normal((rows, heads, d)).astype(np.float32)
+    table = np.tile(np.arange(4, dtype=np.int32), rounds)[None].repeat(rows, 0)
+    x, tab, pos = _up(q), _up(table), _up(np.full(rows, 4 * block * rounds - 1, np.int32))
+    out, lse = torch.empty((rows, heads, d), device="cuda"), torch.empty((rows, heads), device="cuda")
+    jl.Kv8Attention(p.pages, ws, x.data_ptr(), out.data_ptr(), GGMLType.F32, rows=rows, heads=heads, blockTable=tab.data_ptr(), slots=rows,
+                    blocksPerSlot=4 * rounds, positions=pos.data_ptr(), lse=lse.data_ptr()).launch(_stream())
+    codes, scales = p.host()
+    want, want_lse, most = ref.attention_ref(codes, scales, q, table[:, :4], None, np.full(rows, 4 * block - 1), d ** -0.5)
+    torch.cuda.synchronize()
+    tol = 2 * ref.score_tolerance(d, most.max())
+    assert np.linalg.norm(out.cpu().numpy() - want) <= tol * np.linalg.norm(want)
+    # a warp's sum of weights has 2 000 steps of four tokens for a lane, each addition off by 2^-24 of it
+    assert np.abs(lse.cpu().numpy() - want_lse - math.log(rounds)).max() <= tol + 2.0 ** -24 * 4 * 2200 + 2.0 ** -22 * 20
+
+
+@pytest.mark.parametrize("gap", [3.0, 8.0, 12.0, 25.0])
+def test_attention_with_a_token_far_above_the_others(dev, ws, gap):
+    """One token's weight is e^gap times the others': these keep their part of the output, wherever the one stands."""
+    for at in (0, 777, 2999):
+        a = _Attention(dev, ws, rows=1, heads=8, kv_heads=2, d=128, block=16, lengths=[3000], seed=16, spread=0.3, own_slots=True, unwritten=False)
+        codes = a.p.codes
+        b, place = int(a.table[0, at // 16]), at % 16
+        for h in range(2):
+            codes[0, b, h, place] = 100
+            a.p.scales[0, b, h, place] = gap / (100 * 0.3 * 128 ** 0.5) * 128 ** 0.5 / 128
+        a.q[0, :1024] = np.abs(a.q[0, :1024]) + 0.3
+        a.dq.copy_(_up(a.q))
+        a.call().launch(_stream())
+        a.check()
+
+
+@pytest.mark.parametrize("rows", [33, 128, 129, 1000])
+def test_attention_of_many_rows_some_of_them_long(dev, ws, rows):
+    """Rows beyond those that a warp's lanes hold, in front of and behind long ones."""
+    rng = np.random.default_rng(rows)
+    lengths = rng.integers(0, 90, rows)
+    lengths[[0, rows // 2, rows - 1]] = 3000, 5000, 2100
+    a = _Attention(dev, ws, rows=rows, heads=4, kv_heads=2, d=64, block=16, lengths=lengths, seed=rows, rope=True)
+    a.call().launch(_stream())
+    a.check()
+
+
+def test_attention_of_groups_of_more_heads_than_the_grid_has_places(dev, ws):
+    a = _Attention(dev, ws, rows=2, heads=4096, kv_heads=1, d=128, block=16, lengths=[300, 40], seed=17)
+    a.call().launch(_stream())
+    a.check()
+
+
 # ------------------------------------------------------------------------------------------------ calls
+
+@pytest.mark.parametrize("heads,kv_heads,d,block,n", [(6, 6, 192, 48, 700), (12, 2, 96, 7, 5000)])
+def test_the_first_call_of_a_kind_may_be_captured(dev, heads, kv_heads, d, block, n):
+    """Nothing that a first call sets up is in a capture's way; two graphs with one workspace, replayed in turn."""
+    w = jl.Kv8Workspace(dev)
+    a = [_Attention(dev, w, rows=3, heads=heads, kv_heads=kv_heads, d=d, block=block, lengths=[n, 5, n // 2 + k], seed=k) for k in range(2)]
+    graphs = []
+    for x in a:
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g):
+            x.call().launch(torch.cuda.current_stream().cuda_stream)
+        graphs.append(g)
+    for _ in range(3):
+        for x, g in zip(a, graphs):
+            x.out.fill_(77.0)
+            g.replay()
+    for x in a:
+        x.check()
+    del g, graphs
+    w.close()
+
+
+def test_closed_workspaces_and_devices_refuse(dev):
+    d = jl.Device(0)
+    w = jl.Kv8Workspace(d)
+    a = _Attention(d, w, rows=1, heads=4, kv_heads=2, d=64, block=16, lengths=[20])
+    call = a.call()
+    call.launch()
+    d.synchronize()
+    w.close()
+    with pytest.raises(jl.IllegalStateError, match="closed"):
+        call.launch()
+    with jl.Kv8Workspace(d) as again:
+        call.workspace = again
+        call.launch()
+        d.synchronize()
+        d.close()
+        with pytest.raises(jl.IllegalStateError, match="closed"):
+            call.launch()
+    a.check()
+
 
 def test_refused_calls_raise_and_launch_nothing(dev, ws):
     a = _Attention(dev, ws, rows=1, heads=4, kv_heads=2, d=64, block=16, lengths=[20])

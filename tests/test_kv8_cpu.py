@@ -99,6 +99,33 @@ def test_attention_refuses(lib, changes, status, says):
     assert rc == status and says in message
 
 
+def test_calls_without_a_context_refuse(lib):
+    ws = C.c_void_p()
+    assert lib.jl_kv8_workspace_create(None, C.byref(ws)) == 1 and not ws
+    assert lib.jl_kv8_workspace_free(None, None) == 0
+    assert lib.jl_kv8_map(None, None, C.byref(_args(MAP)), None) == 1
+    assert lib.jl_kv8_append(None, C.byref(_args(APPEND)), None) == 1
+    assert lib.jl_kv8_attention(None, None, C.byref(_args(ATTENTION)), None) == 1
+    assert lib.jl_debug_kv8_check(3, None, C.create_string_buffer(8), 8) == 1 and lib.jl_debug_kv8_check(0, None, None, 0) == 1
+
+
+def test_the_kernels_wait_for_what_is_ahead_before_they_touch_memory():
+    """Launched while the kernel ahead still runs, each kernel waits for it before its first access: nothing but its parameters stands in front
+    of the wait, in the text."""
+    import re
+    from pathlib import Path
+    from tests.test_kernel_source_rules import CSRC, _code, _function_at
+    seen = 0
+    for name in ("kv8.cu", "kv8_attention.cu"):
+        text = _code(Path(CSRC) / name)
+        for m in re.finditer(r"__global__", text):
+            body = _function_at(text, m.start())
+            in_front = body[:body.index("pdl_wait()")]
+            assert not re.search(r"a\.\w+\[|\*reinterpret_cast|__ld|\breturn\b", in_front), name
+            seen += 1
+    assert seen == 3
+
+
 def test_plain_map_of_a_small_batch_by_hand():
     """Blocks of 4: a sequence in the middle of a block, one that starts, one that waits, one too long, one beyond the free blocks."""
     table = np.full((5, 3), -1, np.int32)
