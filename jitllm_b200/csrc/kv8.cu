@@ -213,10 +213,12 @@ cudaError_t map_launch(const MapParams &p, int64_t most, int ctas, const Kv8Laun
 // ---- append -------------------------------------------------------------------------------------
 //
 // A row (a token's keys or values of one head) is held by D / 8 lanes, eight elements each, so a warp has one to four rows and reads
-// them in 16-byte pieces. Codes are those of the unrounded values, so that they are a function of the row alone: with 127 x / max |x|
-// in binary32 (off by less than 7e-5: a rotation 2.5, the maximum as much, the quotient 4, of 127 * 2^-24), a row that has an
-// element within 2^-13 of the border of two codes is done again in 64 bits, and so are rows whose largest element is infinite, NaN,
-// above 2^125 or close to 2^-100. That is a row in thirty.
+// them in 16-byte pieces; the lanes take the keys and the values of their token and head, whose places are the same. Codes are
+// those of the unrounded values, so that they are a function of the row alone: 127 x / max |x| in binary32 is off by less than 1.6e-5
+// (the quotient 2 of 127 * 2^-24), rotated by less than 5.3e-5 (the rotation 2.5, the maximum as much), and a row that has an
+// element nearer than 2^-16 (rotated 2^-14) to the border of two codes is done again in 64 bits; so are rows whose largest element is
+// infinite, NaN, above 2^125 or close to 2^-100. That is a row in 250, rotated one in 60.
+// Bound by what it reads: 8191 tokens of 8 heads of 128 in binary32 are 85 MB, 13.2 us at the copy rate.
 
 constexpr int kAppendThreads = 256;
 
@@ -247,7 +249,7 @@ struct Eight<__half> {
 
 struct AppendParams {
     jl_kv8_append_args a;
-    uint64_t divide, divide_rows;  // j / block_tokens = j * divide >> shift for j < 2^31; the same for rows of a token
+    uint64_t divide, divide_rows;  // j / block_tokens = j * divide >> shift for j < 2^31; the same for the heads of a token
     int shift, shift_rows;
 };
 
@@ -258,87 +260,95 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
     const int sub = threadIdx.x % kLanes;
     pdl_launch_dependents();
     pdl_wait();
-    const uint32_t heads = a.pages.kv_heads, row = blockIdx.x * uint32_t(kAppendThreads / kLanes) + threadIdx.x / kLanes;  // rows: token, side, head
-    const uint32_t t = uint32_t((uint64_t(row) * p.divide_rows) >> p.shift_rows), in_token = row - t * 2 * heads;
-    const bool values = in_token >= heads;
-    const uint32_t head = values ? in_token - heads : in_token;
+    const uint32_t heads = a.pages.kv_heads, row = blockIdx.x * uint32_t(kAppendThreads / kLanes) + threadIdx.x / kLanes;  // rows: token, head
+    const uint32_t t = uint32_t((uint64_t(row) * p.divide_rows) >> p.shift_rows), head = row - t * heads;
     const int count = a.token_count ? min(a.token_count[0], a.tokens) : a.tokens;
     const bool here = int64_t(t) < count, mine = here && sub < HD / 8;
+    Eight<T> raw[2] = {};  // keys, values
+    if (mine) {
+        raw[0].load(static_cast<const T *>(a.k) + t * a.k_stride + (head * HD + sub * 8));
+        raw[1].load(static_cast<const T *>(a.v) + t * a.v_stride + (head * HD + sub * 8));
+    }
     const int64_t place = here ? a.slot_map[t] : -1;
-
-    Eight<T> raw = {};
-    if (mine) raw.load(static_cast<const T *>(values ? a.v : a.k) + t * (values ? a.v_stride : a.k_stride) + head * HD + sub * 8);
-    const bool turn = here && !values && a.rope_cos;
-    const int pos = turn ? a.positions[t] : 0;
+    const bool turn = a.rope_cos != nullptr;
+    const int pos = turn && here ? a.positions[t] : 0;
     const bool outside = turn && (pos < 0 || pos >= a.rope_rows);
     float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
     if (turn && !outside && mine) {
         c = *reinterpret_cast<const float4 *>(a.rope_cos + int64_t(pos) * (HD / 2) + sub * 4);
         s = *reinterpret_cast<const float4 *>(a.rope_sin + int64_t(pos) * (HD / 2) + sub * 4);
     }
-    const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
-    float in[8], x[8];
-    raw.get(in);
-    uint32_t bits = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        x[2 * i] = turn ? in[2 * i] * cs[i] - in[2 * i + 1] * sn[i] : in[2 * i];
-        x[2 * i + 1] = turn ? in[2 * i] * sn[i] + in[2 * i + 1] * cs[i] : in[2 * i + 1];
-        bits = max(bits, max(__float_as_uint(x[2 * i]) & 0x7fffffffu, __float_as_uint(x[2 * i + 1]) & 0x7fffffffu));
-    }
-#pragma unroll
-    for (int d = kLanes / 2; d; d >>= 1) bits = max(bits, __shfl_xor_sync(~0u, bits, d));
-    const float most = __uint_as_float(bits), up = __fdividef(127.f, most), magic = 12582912.f;  // 1.5 * 2^23: a sum's low byte is the code
-    float border = 0.f;
-    uint32_t code[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float y = fmaf(x[i], up, magic);
-        border = fmaxf(border, fabsf(fmaf(x[i], up, magic - y)));
-        code[i] = __float_as_uint(y);
-    }
-    const bool again = outside || !(most >= 0x1p-99f && most < 0x1p125f) || border > 0.5f - 0x1p-13f;
-    float scale = most * (1.f / 127.f);
-    // whether any lane of the row says so
-    const unsigned says = __ballot_sync(~0u, again && here);
-    if (says) {
-        const unsigned row_lanes = kLanes == 32 ? ~0u : ((1u << (kLanes & 31)) - 1) << (threadIdx.x & 31 & ~(kLanes - 1));
-        double exact[8], largest = 0;
-        bool good = !outside;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const double u = in[2 * i], w = in[2 * i + 1];
-            exact[2 * i] = turn ? u * double(cs[i]) - w * double(sn[i]) : u;
-            exact[2 * i + 1] = turn ? u * double(sn[i]) + w * double(cs[i]) : w;
-            good = good && isfinite(exact[2 * i]) && isfinite(exact[2 * i + 1]);
-            largest = fmax(largest, fmax(fabs(exact[2 * i]), fabs(exact[2 * i + 1])));
-        }
-        good = (__ballot_sync(~0u, good) & row_lanes) == row_lanes;
-#pragma unroll
-        for (int d = kLanes / 2; d; d >>= 1) largest = fmax(largest, __shfl_xor_sync(~0u, largest, d));
-        if (says & row_lanes) {
-            const bool some = good && largest >= 0x1p-100;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) code[i] = some ? uint32_t(int(rint(exact[i] * 127.0 / largest))) : 0;
-            scale = good ? (some ? float(largest / 127.0) : 0.f) : CUDART_NAN_F;
-        }
-    }
-    if (!mine || place < 0 || place >= int64_t(a.pages.blocks) * a.pages.block_tokens) return;
     // a place may be beyond 31 bits
     const int64_t block = place < 0x7fffffff ? int64_t((uint64_t(place) * p.divide) >> p.shift) : place / a.pages.block_tokens;
     const int64_t at = int64_t(head) * a.pages.block_tokens + (place - block * a.pages.block_tokens);
-    int8_t *to = (values ? a.pages.v : a.pages.k) + block * a.pages.block_stride + at * HD + sub * 8;
-    uint2 packed;
-    packed.x = __byte_perm(__byte_perm(code[0], code[1], 0x0040), __byte_perm(code[2], code[3], 0x0040), 0x5410);
-    packed.y = __byte_perm(__byte_perm(code[4], code[5], 0x0040), __byte_perm(code[6], code[7], 0x0040), 0x5410);
-    *reinterpret_cast<uint2 *>(to) = packed;
-    if (sub == 0) (values ? a.pages.v_scale : a.pages.k_scale)[block * a.pages.scale_stride + at] = scale;
+    const int64_t code_at = block * a.pages.block_stride + at * HD + sub * 8, scale_at = block * a.pages.scale_stride + at;
+    const bool stored = mine && place >= 0 && place < int64_t(a.pages.blocks) * a.pages.block_tokens;
+
+    // side 0: keys, 1: values
+    auto store = [&](const int side) {
+        const bool turned = side == 0 && turn, lost = side == 0 && outside;
+        const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
+        float in[8], x[8];
+        raw[side].get(in);
+        uint32_t bits = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = turned ? in[2 * i] * cs[i] - in[2 * i + 1] * sn[i] : in[2 * i];
+            x[2 * i + 1] = turned ? in[2 * i] * sn[i] + in[2 * i + 1] * cs[i] : in[2 * i + 1];
+            bits = max(bits, max(__float_as_uint(x[2 * i]) & 0x7fffffffu, __float_as_uint(x[2 * i + 1]) & 0x7fffffffu));
+        }
+#pragma unroll
+        for (int d = kLanes / 2; d; d >>= 1) bits = max(bits, __shfl_xor_sync(~0u, bits, d));
+        const float most = __uint_as_float(bits), up = 127.f * __frcp_rn(most), magic = 12582912.f;  // 1.5 * 2^23: a sum's low byte is the code
+        float border = 0.f;
+        uint32_t code[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float y = fmaf(x[i], up, magic);
+            border = fmaxf(border, fabsf(fmaf(x[i], up, magic - y)));
+            code[i] = __float_as_uint(y);
+        }
+        const bool again = lost || !(most >= 0x1p-99f && most < 0x1p125f) || border > 0.5f - (turned ? 0x1p-14f : 0x1p-16f);
+        float scale = most * (1.f / 127.f);
+        // whether any lane of the row says so
+        const unsigned says = __ballot_sync(~0u, again && here);
+        if (says) {
+            const unsigned row_lanes = kLanes == 32 ? ~0u : ((1u << (kLanes & 31)) - 1) << (threadIdx.x & 31 & ~(kLanes - 1));
+            double exact[8], largest = 0;
+            bool good = !lost;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const double u = in[2 * i], w = in[2 * i + 1];
+                exact[2 * i] = turned ? u * double(cs[i]) - w * double(sn[i]) : u;
+                exact[2 * i + 1] = turned ? u * double(sn[i]) + w * double(cs[i]) : w;
+                good = good && isfinite(exact[2 * i]) && isfinite(exact[2 * i + 1]);
+                largest = fmax(largest, fmax(fabs(exact[2 * i]), fabs(exact[2 * i + 1])));
+            }
+            good = (__ballot_sync(~0u, good) & row_lanes) == row_lanes;
+#pragma unroll
+            for (int d = kLanes / 2; d; d >>= 1) largest = fmax(largest, __shfl_xor_sync(~0u, largest, d));
+            if (says & row_lanes) {
+                const bool some = good && largest >= 0x1p-100;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) code[i] = some ? uint32_t(int(rint(exact[i] * 127.0 / largest))) : 0;
+                scale = good ? (some ? float(largest / 127.0) : 0.f) : CUDART_NAN_F;
+            }
+        }
+        if (!stored) return;
+        uint2 packed;
+        packed.x = __byte_perm(__byte_perm(code[0], code[1], 0x0040), __byte_perm(code[2], code[3], 0x0040), 0x5410);
+        packed.y = __byte_perm(__byte_perm(code[4], code[5], 0x0040), __byte_perm(code[6], code[7], 0x0040), 0x5410);
+        *reinterpret_cast<uint2 *>((side ? a.pages.v : a.pages.k) + code_at) = packed;
+        if (sub == 0) (side ? a.pages.v_scale : a.pages.k_scale)[scale_at] = scale;
+    };
+    store(0);
+    store(1);
 }
 
 template <int HD>
 cudaError_t append_launch(const AppendParams &p, const Kv8Launch &l) {
     constexpr int kLanes = HD <= 64 ? 8 : HD <= 128 ? 16 : 32;
-    const int64_t rows = int64_t(p.a.tokens) * p.a.pages.kv_heads * 2;
+    const int64_t rows = int64_t(p.a.tokens) * p.a.pages.kv_heads;
     const unsigned grid = unsigned((rows * kLanes + kAppendThreads - 1) / kAppendThreads);
     return kv8_launch(p.a.ggml_type == JL_F16 ? append_kernel<HD, __half> : append_kernel<HD, float>, grid, kAppendThreads, 0, l.stream, l.programmatic, p);
 }
@@ -369,7 +379,7 @@ cudaError_t kv8_append_launch(const jl_kv8_append_args &a, const Kv8Launch &l) {
     AppendParams p = {};
     p.a = a;
     kv8_division(a.pages.block_tokens, &p.divide, &p.shift);
-    kv8_division(2 * a.pages.kv_heads, &p.divide_rows, &p.shift_rows);
+    kv8_division(a.pages.kv_heads, &p.divide_rows, &p.shift_rows);
     switch (a.pages.head_dim) {
         case 64: return append_launch<64>(p, l);
         case 96: return append_launch<96>(p, l);
