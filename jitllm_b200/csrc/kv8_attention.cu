@@ -33,7 +33,8 @@ constexpr uint32_t kGroup = 32;          // parts that are joined at once
 constexpr int kSlots = 4;                // for parts, of a CTA
 static_assert(kMostCtas <= int(kGroup * kGroup));
 constexpr int kFlush = 2048;             // steps after which sums of 2^14 a token could pass 2^30
-constexpr float kHeadroom = 26.f;        // E moves on so that weights are below 2^27, and again when one would pass 2^30.5
+constexpr float kNothing = -3e38f;       // m and E before there is a token
+constexpr float kHeadroom = 26.f;        // E moves on so that weights are below 2^27, and again when one passes 1.5e9 or could pass 2^30
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 
 // ---- layout of a stage in shared memory: 32 rows of keys, 32 rows of values, their scales, the mask of tokens that count -----------
@@ -114,7 +115,7 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// 2^(from - to) of whole numbers from <= to, exactly (from -inf: nothing is there, 0; below 2^-126: 0)
+// 2^(from - to) of whole numbers from <= to, exactly (below 2^-126, and from kNothing: 0)
 __device__ __forceinline__ float step_down(float from, float to) {
     const float magic = 12582912.f;  // 1.5 * 2^23: the sum's low bits are the whole number
     return from == to ? 1.f : __int_as_float((__float_as_int(fmaxf(from - to, -127.f) + magic) - __float_as_int(magic) + 127) << 23);
@@ -452,8 +453,8 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
     auto finish = [&](int f, int row, int kv, float4 x, float top, float etop, float sum) {
         const int head = 4 * (f / L::kQuads) + t;
         if (head0 + head >= p.group) return;
-        // 2^(etop - top) / sum, in two factors: either may be beyond binary32 where the output is not. etop is above top - 160 and
-        // below top + 110, since a scale's exponent is between -126 and 128.
+        // 2^(etop - top) / sum, in two factors: either may be beyond binary32 where the output is not. The two are less than 200 apart:
+        // a scale's exponent is between -126 and 128, E within 30 of the largest weight's, m within 20 of the largest score.
         const float inverse = sum == 0.f ? 0.f : 1.f / sum;
         const int power = sum == 0.f || !(fabsf(etop - top) < 200.f) ? 0 : int(etop - top), h1 = power / 2;
         const float f1 = inverse * __int_as_float((127 + h1) << 23), f2 = __int_as_float((127 + power - h1) << 23);
@@ -545,7 +546,7 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
         int since = 0;                     // steps in `acc`
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            m[n] = e[n] = -CUDART_INF_F;
+            m[n] = e[n] = kNothing;
             l[n] = 0.f;
 #pragma unroll
             for (int j = 0; j < L::kQuads; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
@@ -597,52 +598,58 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
                 }
             }
 
-            // scores in units of ln 2, weights as mantissa and exponent of the value's scale
+            // scores in units of ln 2 and weights
             const unsigned mask = *reinterpret_cast<const unsigned *>(stage + L::kMask) >> g;
             const float *ks = reinterpret_cast<const float *>(stage + L::kScales) + g, *vs = ks + kStep;
-            float mantissa[4], exponent[4];
+            float v[4];
+            bool odd_scale = false;  // beyond 2^-60 .. 2^60: exponents are taken apart below
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const float v = mask >> (8 * k) & 1 ? vs[8 * k] : 0.f;
-                const uint32_t bits = __float_as_uint(v), ex = bits >> 23 & 255;
-                bad = bad || ex == 255;
-                mantissa[k] = ex ? __uint_as_float((bits & 0x807fffffu) | 0x3f800000u) : v * 0x1p126f;
-                exponent[k] = __uint_as_float(0x4b000000u | max(ex, 1u)) - 8388735.f;  // 2^23 + 127
+                v[k] = mask >> (8 * k) & 1 ? vs[8 * k] : 1.f;
+                odd_scale = odd_scale || (__float_as_uint(v[k]) & 0x7fffffffu) - 0x21800000u > 0x5d800000u - 0x21800000u;
             }
             uint32_t w[NT][2][2];  // columns as of the queries; groups of tokens t and t + 4
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                float x[4];
-                bool beyond = false;
+                float x[4], y[4];
+                bool beyond = odd_scale;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const int(&c)[2][4] = s[n][k >> 1];
                     const int at2 = 2 * (k & 1);
                     const float dot = fmaf(float(c[0][at2] * 256 + c[0][at2 + 1]), 65536.f, float(c[1][at2] * 256 + c[1][at2 + 1]));
                     x[k] = mask >> (8 * k) & 1 ? dot * factor[n] * ks[8 * k] : -CUDART_INF_F;
-                    beyond = beyond || x[k] - m[n] > 20.f || x[k] - e[n] + exponent[k] > 29.5f;
+                    y[k] = exp2_approx(x[k] - e[n]) * v[k];
+                    beyond = beyond || x[k] - m[n] > 20.f || fabsf(y[k]) > 1.5e9f;
                 }
                 if (__any_sync(~0u, beyond)) {
-                    float top = -CUDART_INF_F, etop = -CUDART_INF_F;
+                    float mantissa[4], exponent[4], top = kNothing, etop = kNothing;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) top = fmaxf(top, x[k]), etop = fmaxf(etop, x[k] + exponent[k]);
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t bits = __float_as_uint(v[k]), ex = bits >> 23 & 255;
+                        bad = bad || ex == 255;
+                        mantissa[k] = ex ? __uint_as_float((bits & 0x807fffffu) | 0x3f800000u) : v[k] * 0x1p126f;
+                        exponent[k] = __uint_as_float(0x4b000000u | max(ex, 1u)) - 8388735.f;  // 2^23 + 127
+                        top = fmaxf(top, x[k]), etop = fmaxf(etop, x[k] + exponent[k]);
+                    }
 #pragma unroll
                     for (int d = 4; d < 32; d <<= 1) {
                         top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
                         etop = fmaxf(etop, __shfl_xor_sync(~0u, etop, d));
                     }
-                    const float m_new = fmaxf(m[n], ceilf(top)), e_new = fmaxf(e[n], ceilf(etop) - kHeadroom), keep = step_down(e[n], e_new);
+                    const float m_new = top - m[n] > 20.f ? ceilf(top) : m[n], e_new = etop - e[n] > 29.f ? ceilf(etop) - kHeadroom : e[n], keep = step_down(e[n], e_new);
                     l[n] *= step_down(m[n], m_new);
                     if (i > 0 && __any_sync(~0u, keep != 1.f)) flush(n, keep);
                     m[n] = m_new;
                     e[n] = e_new;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) y[k] = exp2_approx(x[k] - e[n] + exponent[k]) * mantissa[k];
                 }
                 uint32_t bytes[4], digit[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    // where nothing has been seen yet, m = E = -inf, which -inf may not be taken from; NaN becomes 0
-                    l[n] += x[k] == -CUDART_INF_F ? 0.f : exp2_approx(x[k] - m[n]);
-                    bytes[k] = signed_bytes(__float2int_rn(exp2_approx(x[k] - e[n] + exponent[k]) * mantissa[k]));
+                    l[n] += exp2_approx(x[k] - m[n]);
+                    bytes[k] = signed_bytes(__float2int_rn(y[k]));  // NaN becomes 0
                 }
                 transpose_bytes(bytes, digit);
                 // lane (g, t) has the words of head t and tokens g; column g is of head g / 2
