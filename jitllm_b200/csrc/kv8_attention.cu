@@ -120,8 +120,13 @@ __device__ __forceinline__ float step_down(float from, float to) {
     const float magic = 12582912.f;  // 1.5 * 2^23: the sum's low bits are the whole number
     return from == to ? 1.f : __int_as_float((__float_as_int(fmaxf(from - to, -127.f) + magic) - __float_as_int(magic) + 127) << 23);
 }
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, uint64_t policy) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy) : "memory");
+}
+__device__ __forceinline__ uint64_t policy_normal() {
+    uint64_t policy;
+    asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
+    return policy;
 }
 // SIZE bytes, or as many zeros
 template <int SIZE>
@@ -335,6 +340,8 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
         code_at = good ? block * a.pages.block_stride + in_block * HD : -1;
         scale_at = good ? block * a.pages.scale_stride + in_block : -1;
     };
+    // Codes that no other CTA wants are the first to leave L2 (16 rows at 32000: 187 / 194 us with / without, head size 64 97 / 113).
+    const uint64_t policy = p.head_tiles == 1 ? policy_evict_first() : policy_normal();
     // Keys, scales and mask of step i, and its values, as groups of copies of their own.
     auto copy_rows = [&](int i, const int8_t *pages, uint32_t stage) {
         if constexpr (PAGED16) {
@@ -346,7 +353,7 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
 #pragma unroll
                     for (int n = 0; n < HD / 32; ++n) {
                         const int piece16 = n * 32 + lane;
-                        copy16(stage + L::piece(16 * half + piece16 / (HD / 16), piece16 % (HD / 16)), src + n * 512);
+                        copy16(stage + L::piece(16 * half + piece16 / (HD / 16), piece16 % (HD / 16)), src + n * 512, policy);
                     }
                 }
             }
@@ -355,7 +362,7 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
             for (int n = 0; n < HD / 16; ++n) {
                 const int piece16 = n * 32 + lane, row32 = piece16 / (HD / 16), c = piece16 % (HD / 16);
                 const int64_t src = __shfl_sync(~0u, code_at, row32);
-                if (src >= 0) copy16(stage + L::piece(row32, c), pages + src + c * 16);
+                if (src >= 0) copy16(stage + L::piece(row32, c), pages + src + c * 16, policy);
             }
         }
     };
@@ -885,8 +892,11 @@ cudaError_t launch(Params &p, const Kv8Scratch &s, const Kv8Launch &l) {
 template <int HD>
 cudaError_t launch_head(Params &p, const Kv8Scratch &s, const Kv8Launch &l) {
     const bool paged16 = p.a.pages.block_tokens % 16 == 0;
+    // More than four query heads of a KV head: eight to a unit, or four, whose CTAs then read a token's keys and values twice (from L2 the
+    // second time). Head size 128, eight heads, four and eight to a unit (us): 8 rows at 2000 of 8 KV heads 21.2 / 24.2, at 16000 76 / 88, 1 row at
+    // 100000 of one 21.1 / 26.3; but 32 rows at 300 20.6 / 17.4, where units are many. Head size 64: 16 rows at 16000 of 4 KV heads 53.3 / 50.2.
     if constexpr (HD <= 128)
-        if (p.group > 4) return paged16 ? launch<HD, 2, true>(p, s, l) : launch<HD, 2, false>(p, s, l);
+        if (p.group > 4 && (HD == 64 || int64_t(p.a.rows) * p.a.pages.kv_heads >= l.sm_count)) return paged16 ? launch<HD, 2, true>(p, s, l) : launch<HD, 2, false>(p, s, l);
     return paged16 ? launch<HD, 1, true>(p, s, l) : launch<HD, 1, false>(p, s, l);
 }
 
