@@ -302,7 +302,7 @@ typedef struct {
     int32_t blocks, block_tokens, kv_heads, head_dim;
 } jl_kv8_pages;
 
-/* Device memory that jl_kv8_map and jl_kv8_attention keep their partial results and arrival counters in: about 10 MB, made once.
+/* Device memory that jl_kv8_map and jl_kv8_attention keep their partial results and arrival counters in: about 5 MB, made once, not while a stream is being captured.
  * Calls with one workspace must not overlap on the GPU: one workspace for each stream (or captured graph) that runs beside
  * others. Calls of any shape may follow one another. Free it when no call with it is under way and no graph holds one. */
 typedef struct jl_kv8_workspace jl_kv8_workspace;

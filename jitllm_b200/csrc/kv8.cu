@@ -19,6 +19,8 @@ namespace {
 // sequences, 64 KB from L2) and keeps them in shared memory; then tokens and blocks are dealt out evenly, whatever the
 // sequences' lengths. So there is one launch and nothing to wait for between CTAs. What may be an input and an output at once
 // (lengths, cursor) is written by the CTA that is through last.
+// Bound by the chain of loads, sums and searches, not by bytes: 8 sequences 3.3 us, 201 sequences with 3 800 tokens 4.2 us, 4096 sequences
+// with 10^6 tokens (16.3 MB) 14.1 us. One token for each thread, and four in a row with wide stores: 3.3 / 4.6, 4.2 / 6.7, 15.0 / 14.1 us.
 
 constexpr int kMapThreads = 512;
 constexpr int kMapWarps = kMapThreads / 32;
@@ -218,7 +220,8 @@ cudaError_t map_launch(const MapParams &p, int64_t most, int ctas, const Kv8Laun
 // (the quotient 2 of 127 * 2^-24), rotated by less than 5.3e-5 (the rotation 2.5, the maximum as much), and a row that has an
 // element nearer than 2^-16 (rotated 2^-14) to the border of two codes is done again in 64 bits; so are rows whose largest element is
 // infinite, NaN, above 2^125 or close to 2^-100. That is a row in 250, rotated one in 60.
-// Bound by what it reads: 8191 tokens of 8 heads of 128 in binary32 are 85 MB, 13.2 us at the copy rate.
+// Bound by what it reads, and by its instructions (about 15 for an element): 8191 tokens of 8 heads of 128 in binary32, 84.5 MB, take 19.6 us =
+// 4.3 TB/s, 0.67 of the measured copy rate; a row for each side by lanes of its own took 28.6 us. A single token takes 2.2 us.
 
 constexpr int kAppendThreads = 256;
 
