@@ -288,7 +288,8 @@ const char *jl_static_last_error(void);
  * cudaStream_t of that GPU; NULL is the default stream, jl_stream(ctx) the context's own) and returns without waiting; none
  * allocates or synchronises, so all may be captured into CUDA graphs. The argument structure is read during the call only.
  * What the device finds wrong (an index beyond its bounds) is passed over as described at each field; it never leads to an
- * access outside the buffers described. The current device is left as it was. */
+ * access outside the buffers described. No output may overlap an input or another output, but for those of jl_kv8_map that say
+ * which input they may be. The current device is left as it was. */
 
 /* Pages. Block b of keys (values) starts block_stride bytes (elements) behind block b - 1 and holds
  * int8 [kv_heads][block_tokens][head_dim]; its scales start scale_stride floats behind those of block b - 1 and are

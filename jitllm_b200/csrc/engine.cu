@@ -2271,7 +2271,13 @@ int32_t jl_kv8_workspace_create(jl_ctx *ctx, jl_kv8_workspace **out) {
         delete ws;
         return fail(ctx, e == cudaErrorMemoryAllocation ? JL_ERR_OOM : JL_ERR_CUDA, "workspace allocation failed: %s", cudaGetErrorString(e));
     }
-    ctx->kv8_workspaces.push_back(ws);
+    try {
+        ctx->kv8_workspaces.push_back(ws);
+    } catch (const std::bad_alloc &) {  // no exception may leave a C entry
+        kv8_scratch_free(&ws->scratch);
+        delete ws;
+        return fail(ctx, JL_ERR_OOM, "host memory exhausted");
+    }
     *out = ws;
     return JL_OK;
 }
@@ -2306,7 +2312,10 @@ int32_t jl_kv8_map(jl_ctx *ctx, jl_kv8_workspace *ws, const jl_kv8_map_args *arg
     JL_REQUIRE(ctx, owns(ctx, ws), JL_ERR_INVALID, "the workspace is not one of this context's");
     DeviceGuard guard(ctx->device);
     const cudaError_t e = kv8_map_launch(*args, ws->scratch, {ctx->sm_count, ctx->use_pdl, static_cast<cudaStream_t>(stream)});
-    if (e != cudaSuccess) return fail(ctx, JL_ERR_CUDA, "block map launch failed: %s", cudaGetErrorString(e));
+    if (e != cudaSuccess) {
+        cudaGetLastError();  // the caller is told; the next launch's check is not to find it again
+        return fail(ctx, JL_ERR_CUDA, "block map launch failed: %s", cudaGetErrorString(e));
+    }
     ctx->counters.kernel_launches++;
     return JL_OK;
 }
@@ -2319,7 +2328,10 @@ int32_t jl_kv8_append(jl_ctx *ctx, const jl_kv8_append_args *args, void *stream)
     if (args->tokens == 0) return JL_OK;
     DeviceGuard guard(ctx->device);
     const cudaError_t e = kv8_append_launch(*args, {ctx->sm_count, ctx->use_pdl, static_cast<cudaStream_t>(stream)});
-    if (e != cudaSuccess) return fail(ctx, JL_ERR_CUDA, "append launch failed: %s", cudaGetErrorString(e));
+    if (e != cudaSuccess) {
+        cudaGetLastError();  // the caller is told; the next launch's check is not to find it again
+        return fail(ctx, JL_ERR_CUDA, "append launch failed: %s", cudaGetErrorString(e));
+    }
     ctx->counters.kernel_launches++;
     return JL_OK;
 }
@@ -2333,7 +2345,10 @@ int32_t jl_kv8_attention(jl_ctx *ctx, jl_kv8_workspace *ws, const jl_kv8_attenti
     if (args->rows == 0) return JL_OK;
     DeviceGuard guard(ctx->device);
     const cudaError_t e = kv8_attention_launch(*args, ws->scratch, {ctx->sm_count, ctx->use_pdl, static_cast<cudaStream_t>(stream)});
-    if (e != cudaSuccess) return fail(ctx, JL_ERR_CUDA, "attention launch failed: %s", cudaGetErrorString(e));
+    if (e != cudaSuccess) {
+        cudaGetLastError();  // the caller is told; the next launch's check is not to find it again
+        return fail(ctx, JL_ERR_CUDA, "attention launch failed: %s", cudaGetErrorString(e));
+    }
     ctx->counters.kernel_launches++;
     return JL_OK;
 }

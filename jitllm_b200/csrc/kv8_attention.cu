@@ -206,7 +206,7 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
     const int rows = a.token_count ? min(a.token_count[0], a.rows) : a.rows;
 
     // ---- what this CTA takes. Short lines: a piece of one unit, every unit cut into equal pieces of `quota` tiles at most, as
-    // many as there are CTAs. Long ones, and more rows than a warp holds: [at, end) of the line, cut without regard to units.
+    // many as there are CTAs. Long ones, and more rows than four for each lane: [at, end) of the line, cut without regard to units.
     // Where a KV head has more query heads than a unit, neighbouring CTAs take the same tokens for their own heads at the same time,
     // and all but the first read them from L2.
     const uint32_t head_tile = blockIdx.x % p.head_tiles, cta = blockIdx.x / p.head_tiles;
