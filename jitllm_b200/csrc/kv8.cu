@@ -220,10 +220,13 @@ cudaError_t map_launch(const MapParams &p, int64_t most, int ctas, const Kv8Laun
 // (the quotient 2 of 127 * 2^-24), rotated by less than 5.3e-5 (the rotation 2.5, the maximum as much), and a row that has an
 // element nearer than 2^-16 (rotated 2^-14) to the border of two codes is done again in 64 bits; so are rows whose largest element is
 // infinite, NaN, above 2^125 or close to 2^-100. That is a row in 250, rotated one in 60.
-// Bound by what it reads, and by its instructions (about 15 for an element): 8191 tokens of 8 heads of 128 in binary32, 84.5 MB, take 19.6 us =
-// 4.3 TB/s, 0.67 of the measured copy rate; a row for each side by lanes of its own took 28.6 us. A single token takes 2.2 us.
+// Bound by what it reads, and by its instructions (23 for an element, issued in 0.66 of the cycles): 8191 tokens of 8 heads of 128 in
+// binary32, 84.5 MB, take 18.3 us = 4.6 TB/s, 0.72 of the measured copy rate; a row for each side by lanes of its own took 28.6 us. A
+// single token takes 2.2 us.
 
-constexpr int kAppendThreads = 256;
+// Nine CTAs of 128 threads per SM, 56 registers each: those 8191 tokens took 18.8 us with 62 to 64 registers (eight CTAs), 18.5 with 48 and
+// spills outside the second look, 19.5 as four CTAs of 256 threads.
+constexpr int kAppendThreads = 128;
 
 template <typename T>
 struct Eight;
@@ -257,7 +260,7 @@ struct AppendParams {
 };
 
 template <int HD, typename T>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kAppendThreads, 9) append_kernel(const AppendParams p) {
     constexpr int kLanes = HD <= 64 ? 8 : HD <= 128 ? 16 : 32;  // HD / 8 of them have elements
     const jl_kv8_append_args &a = p.a;
     const int sub = threadIdx.x % kLanes;
