@@ -360,7 +360,9 @@ int32_t jl_kv8_append(jl_ctx *ctx, const jl_kv8_append_args *args, void *stream)
  * lse = ln sum exp(scale * q.k). Queries are rotated like the keys of jl_kv8_append if rope tables are given (a position
  * beyond them makes the row NaN). Tokens beyond the table's row, and tokens whose table entry is no block of the pages, have no
  * weight. A row that attends to nothing (position -1, a sequence outside 0..slots - 1) gets zeros and lse -inf; rows from
- * *token_count on are left as they are. A NaN scale, query or key makes NaN of the outputs that it has weight in. */
+ * *token_count on are left as they are. A NaN scale, query or key makes NaN of the outputs that it has weight in. Scores and sums are
+ * binary32 (scale times a query times codes has to be finite in it); a token's softmax weight times its scale is taken to 2^-18 of
+ * itself where it is within 2^-39 of the largest of its sequence, and smaller ones lose 2^-13 of an output together at most. */
 typedef struct {
     jl_kv8_pages pages;
     const void *q;                  /* [rows], 16-byte aligned, row stride in elements a multiple of 16 bytes */

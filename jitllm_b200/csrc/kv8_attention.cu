@@ -8,11 +8,18 @@
 //
 // Mathematics. s = scale * ks_j * (q . kc_j), weights p_j = 2^(s_j log2 e - m) with a running reference m, and
 // out = sum p_j vs_j vc_j / sum p_j. Both products are of integers: a query is rounded to 31 bits of its head's largest element and
-// cut into four signed bytes (a balanced radix of 256), and so is the weight w_j = 2^(s_j log2 e - E) vs_j, with a power of two E that
-// moves on when a weight would pass 2^30. The four bytes of four heads are the columns of two mma.m16n8k32 (int8, sums in int32), whose
-// rows are tokens (keys) or elements (values): the codes go in as they are, without a conversion (values after a transpose of
-// four by four bytes), and the sums are exact. E follows the weights with the scale, so scales of values may differ by any factor
-// between tokens; m and E are whole numbers, so that moving them on rounds nothing.
+// cut into four signed bytes (a balanced radix of 256), and so is the whole part of the weight w_j = 2^(s_j log2 e - E) vs_j, with a power
+// of two E that moves on when a weight would pass 2^30. Its fraction has four bytes more, 15 bits in each two. Two bytes of four heads are
+// the columns of an mma.m16n8k32 (int8, sums in int32), whose rows are tokens (keys) or elements (values): the codes go in as they
+// are, without a conversion (values after a transpose of four by four bytes), and a step's sums are exact. E follows the weights with
+// the scale, so scales of values may differ by any factor between tokens; m and E are whole numbers, so that moving them on rounds nothing.
+//
+// What small weights keep. A token far above the others says nothing about an element where its code is 0; that is made up of the
+// others, whose weights must not drown in the digits of the large one. A warp's largest weight times scale is above 2^26, so one within
+// 2^-39 of it (27 nats) is cut off by less than 2^-18 of itself. What the smaller ones lose is added up, and where it could be more than
+// 2^-13 of an output, the warp goes over its tokens again for the digits behind those. Whole numbers alone, which lose a weight
+// of 2^-28 of the largest, took (us) 184 for 16 rows at 32000, 11.2 for one row at 3901, 12.6 for 32 rows at 512, 18.2 for 64 rows with a window
+// of 1000; these take 172, 11.6, 13.7 and 20.8. A second pass doubles them: 66 us in place of 49 for 16 rows at 2000 of head size 256 and scores of 3 nats.
 //
 // What bounds it (kernel alone, back to back; copy rate 6.46 TB/s). 16 rows at 32000 tokens of 8 KV heads of 128, 1.08 GB: 186 us, 5.8 TB/s; with
 // equal pieces the SMs are through between 0.85 and 1.15 of the mean, since they do not get their data at one rate. 64 rows with a
@@ -44,6 +51,9 @@ static_assert(kMostCtas <= int(kGroup * kGroup));
 constexpr int kFlush = 2048;             // steps after which sums of 2^14 a token could pass 2^30
 constexpr float kNothing = -3e38f;       // m and E before there is a token
 constexpr float kHeadroom = 26.f;        // E moves on so that weights are below 2^27, and again when one passes 1.5e9 or could pass 2^30
+constexpr float kDeep = 0x1p2f, kLow = kDeep * 0x1p-15f;  // weights that are off by 2^-18 of themselves at most with 15 bits of their fraction, and with 30
+constexpr float kLoss = 0x1p-13f;        // of an output, that weights below the second may lose
+constexpr float kMagic = 12582912.f;     // 1.5 * 2^23: a sum's low bits are those of the whole number, to the nearest
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 
 // ---- layout of a stage in shared memory: 32 rows of keys, 32 rows of values, their scales, the mask of tokens that count -----------
@@ -126,8 +136,7 @@ __device__ __forceinline__ float exp2_approx(float x) {
 }
 // 2^(from - to) of whole numbers from <= to, exactly (below 2^-126, and from kNothing: 0)
 __device__ __forceinline__ float step_down(float from, float to) {
-    const float magic = 12582912.f;  // 1.5 * 2^23: the sum's low bits are the whole number
-    return from == to ? 1.f : __int_as_float((__float_as_int(fmaxf(from - to, -127.f) + magic) - __float_as_int(magic) + 127) << 23);
+    return from == to ? 1.f : __int_as_float((__float_as_int(fmaxf(from - to, -127.f) + kMagic) - __float_as_int(kMagic) + 127) << 23);
 }
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, uint64_t policy) {
     asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy) : "memory");
@@ -557,37 +566,37 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
         // ---- one pass over this warp's tokens: lane (g, t) has tokens g, g + 8, g + 16, g + 24 of a step, heads 4 n + t, elements of
         // column g. The four tokens of g are bytes of one word of weights, and so are those of t and of t + 4 in a word of values.
         float m[NT], e[NT], l[NT], o[NT][L::kQuads][4];
-        int acc[NT][2 * L::kQuads][2][4];  // elements 2 i and 2 i + 1 of a word; bytes 3 and 2, 1 and 0
-        bool bad = false;                  // a value's scale was no number
-        int since = 0;                     // steps in `acc`
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            m[n] = e[n] = kNothing;
-            l[n] = 0.f;
-#pragma unroll
-            for (int j = 0; j < L::kQuads; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
-#pragma unroll
-            for (int j = 0; j < 2 * L::kQuads; ++j)
-#pragma unroll
-                for (int b = 0; b < 2; ++b) acc[n][j][b][0] = acc[n][j][b][1] = acc[n][j][b][2] = acc[n][j][b][3] = 0;
-        }
-        // o = (o + acc) keep, acc = 0
+        int acc[NT][2 * L::kQuads][4];  // elements 2 i and 2 i + 1 of a word; bytes 3 and 2 of the weights
+        float loss[NT];                 // of weights below kLow
+        bool bad = false;               // a value's scale was no number
+        int since, pass = 0;            // steps in `acc`; passes over the tokens in front of this one
+        float unit = 1.f;               // of this pass's weights, next to 2^E
+        volatile float sums[NT * L::kQuads * 4];  // of the passes in front
+        auto rest = [](float x) { return fmaf(x, 0x1p15f, kMagic - fmaf(x, 0x1p15f, kMagic)); };  // what a fraction's next 15 bits leave: exact
+        // o = (o + acc) keep, acc = 0; the other bytes' products are in `o` already
         auto flush = [&](int n, float keep) {
 #pragma unroll
             for (int j = 0; j < 2 * L::kQuads; ++j)
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    int(&c)[2][4] = acc[n][j];
-                    float x;
-                    if (since <= 8)  // below 2^22 each: two fit one number
-                        x = fmaf(float(c[0][2 * k] * 256 + c[0][2 * k + 1]), 65536.f, float(c[1][2 * k] * 256 + c[1][2 * k + 1]));
-                    else
-                        x = fmaf(fmaf(fmaf(float(c[0][2 * k]), 256.f, float(c[0][2 * k + 1])), 256.f, float(c[1][2 * k])), 256.f, float(c[1][2 * k + 1]));
+                    int(&c)[4] = acc[n][j];
+                    const float x = since <= 8 ? float(c[2 * k] * 256 + c[2 * k + 1]) : fmaf(float(c[2 * k]), 256.f, float(c[2 * k + 1]));  // below 2^22 each: two fit one number
                     float &y = o[n][j / 2][2 * (j & 1) + k];
-                    y = (y + x) * keep;
-                    c[0][2 * k] = c[0][2 * k + 1] = c[1][2 * k] = c[1][2 * k + 1] = 0;
+                    y = fmaf(x, 65536.f * unit, y) * keep;
+                    c[2 * k] = c[2 * k + 1] = 0;
                 }
         };
+    again:
+        since = 0;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            m[n] = e[n] = kNothing;
+            l[n] = loss[n] = 0.f;
+#pragma unroll
+            for (int j = 0; j < L::kQuads; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
+#pragma unroll
+            for (int j = 0; j < 2 * L::kQuads; ++j) acc[n][j][0] = acc[n][j][1] = acc[n][j][2] = acc[n][j][3] = 0;
+        }
         // A step's keys are free when its scores are done, its values when they are added: both are refilled then, kStages steps ahead.
         issue_keys(S::kStages - 1);
         issue_values(S::kStages - 1);
@@ -618,16 +627,19 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
             const unsigned mask = *reinterpret_cast<const unsigned *>(stage + L::kMask) >> g;
             const float *ks = reinterpret_cast<const float *>(stage + L::kScales) + g, *vs = ks + kStep;
             float v[4];
-            bool odd_scale = false;  // beyond 2^-60 .. 2^60: exponents are taken apart below
+            bool odd_scale = false;  // beyond 2^-60 .. 2^26: exponents are taken apart below, so that no exponential is lost in front of a large scale
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 v[k] = mask >> (8 * k) & 1 ? vs[8 * k] : 1.f;
-                odd_scale = odd_scale || (__float_as_uint(v[k]) & 0x7fffffffu) - 0x21800000u > 0x5d800000u - 0x21800000u;
+                odd_scale = odd_scale || (__float_as_uint(v[k]) & 0x7fffffffu) - 0x21800000u > 0x4c800000u - 0x21800000u;
             }
-            uint32_t w[NT][2][2];  // columns as of the queries; groups of tokens t and t + 4
+            float y[NT][4], keep[NT];
+            float least = kDeep;  // of the weights
+            bool moved = false;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                float x[4], y[4];
+                float x[4];
+                keep[n] = 1.f;
                 bool beyond = odd_scale;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
@@ -635,8 +647,8 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
                     const int at2 = 2 * (k & 1);
                     const float dot = fmaf(float(c[0][at2] * 256 + c[0][at2 + 1]), 65536.f, float(c[1][at2] * 256 + c[1][at2 + 1]));
                     x[k] = mask >> (8 * k) & 1 ? dot * factor[n] * ks[8 * k] : -CUDART_INF_F;
-                    y[k] = exp2_approx(x[k] - e[n]) * v[k];
-                    beyond = beyond || x[k] - m[n] > 20.f || fabsf(y[k]) > 1.5e9f;
+                    y[n][k] = exp2_approx(x[k] - e[n]) * v[k];
+                    beyond = beyond || x[k] - m[n] > 20.f || fabsf(y[n][k]) > 1.5e9f;
                 }
                 if (__any_sync(~0u, beyond)) {
                     float mantissa[4], exponent[4], top = kNothing, etop = kNothing;
@@ -653,30 +665,76 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
                         top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
                         etop = fmaxf(etop, __shfl_xor_sync(~0u, etop, d));
                     }
-                    const float m_new = top - m[n] > 20.f ? ceilf(top) : m[n], e_new = etop - e[n] > 29.f ? ceilf(etop) - kHeadroom : e[n], keep = step_down(e[n], e_new);
+                    const float m_new = top - m[n] > 20.f ? ceilf(top) : m[n], e_new = etop - e[n] > 29.f ? ceilf(etop) - kHeadroom : e[n];
                     l[n] *= step_down(m[n], m_new);
-                    if (i > 0 && __any_sync(~0u, keep != 1.f)) flush(n, keep);
+                    keep[n] = step_down(e[n], e_new);
+                    moved = moved || __any_sync(~0u, keep[n] != 1.f);
                     m[n] = m_new;
                     e[n] = e_new;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) y[k] = exp2_approx(x[k] - e[n] + exponent[k]) * mantissa[k];
+                    for (int k = 0; k < 4; ++k) y[n][k] = exp2_approx(x[k] - e[n] + exponent[k]) * mantissa[k];
                 }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) l[n] += exp2_approx(x[k] - m[n]);
+                for (int times = 0; times < pass; ++times)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) y[n][k] = rest(rest(y[n][k] - float(__float2int_rn(y[n][k])))) * 0x1p26f;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) least = fminf(least, fabsf(y[n][k]));
+            }
+            // The fraction's second 15 bits only where a weight is below 4, or always: head size 64, 64 rows with a window of 1000 20.8 / 22.1 us; 128, 16
+            // rows at 32000 187 / 172 and 32 rows at 512 13.6 / 13.9, with scores of twice the size 206 / 178 and 15.0 / 14.2.
+            const bool deep = HD > 64 || __any_sync(~0u, least < kDeep);
+            if (moved || since == kFlush) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) flush(n, keep[n]);
+                since = 0;
+            }
+            ++since;
+            // The columns, as of the queries: of whole numbers (two pairs of bytes), of their fractions' first 15 bits, and of the next 15 where they
+            // count. Lane (g, t) has the bytes of head t and tokens g; column g is of head g / 2; groups of tokens t and t + 4.
+            uint32_t w[NT][4][2];
+            auto columns = [&](const uint32_t (&bytes)[4], int n, int high, int b) {
+#pragma unroll
+                for (int far = 0; far < 2; ++far) {
+                    const int from = (t + 4 * far) * 4 + (g >> 1);
+                    const uint32_t even = __shfl_sync(~0u, bytes[high], from), odd = __shfl_sync(~0u, bytes[high - 1], from);
+                    w[n][b][far] = g & 1 ? odd : even;
+                }
+            };
+            auto fraction_columns = [&](const float (&x)[4], int n, int b) {
+                uint32_t sums[4], digit[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) sums[k] = __float_as_uint(fmaf(x[k], 0x1p15f, kMagic + 128.f));  // of two signed bytes, the second and 128
+                transpose_bytes(sums, digit);
+                digit[0] ^= 0x80808080u;
+                columns(digit, n, 1, b);
+            };
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
                 uint32_t bytes[4], digit[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    l[n] += exp2_approx(x[k] - m[n]);
-                    bytes[k] = signed_bytes(__float2int_rn(y[k]));  // NaN becomes 0
+                    const int whole = __float2int_rn(y[n][k]);  // NaN becomes 0
+                    y[n][k] -= float(whole);                    // exact; 0 from 2^23 on
+                    bytes[k] = signed_bytes(whole);
                 }
                 transpose_bytes(bytes, digit);
-                // lane (g, t) has the words of head t and tokens g; column g is of head g / 2
+                columns(digit, n, 3, 0);
+                columns(digit, n, 1, 1);
+                fraction_columns(y[n], n, 2);
+            }
+            if (deep) {
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
+                for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                    for (int far = 0; far < 2; ++far) {
-                        const int from = (t + 4 * far) * 4 + (g >> 1);
-                        const uint32_t even = __shfl_sync(~0u, digit[3 - 2 * b], from), odd = __shfl_sync(~0u, digit[2 - 2 * b], from);
-                        w[n][b][far] = g & 1 ? odd : even;
+                    for (int k = 0; k < 4; ++k) {
+                        // of the fraction's bits; where there is a whole number in front of them the loss is less
+                        loss[n] += fabsf(y[n][k]) < kLow ? fminf(fabsf(y[n][k]), 0x1p-31f) : 0.f;
+                        y[n][k] = rest(y[n][k]);
                     }
+                    fraction_columns(y[n], n, 3);
+                }
             }
 
             __syncwarp();  // every lane has read keys and scales
@@ -692,44 +750,90 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
                 for (int k = 0; k < 4; ++k) {
                     const unsigned char *at_near = stage + L::kValues + L::piece(t + 8 * k, el >> 4) + (el & 15), *at_far = stage + L::kValues + L::piece(t + 4 + 8 * k, el >> 4) + (el & 15);
                     if constexpr (L::kLoad == 2) {
-                        const uint2 x = *reinterpret_cast<const uint2 *>(at_near), y = *reinterpret_cast<const uint2 *>(at_far);
-                        near[0][k] = x.x, near[1][k] = x.y, far[0][k] = y.x, far[1][k] = y.y;
+                        const uint2 x = *reinterpret_cast<const uint2 *>(at_near), z = *reinterpret_cast<const uint2 *>(at_far);
+                        near[0][k] = x.x, near[1][k] = x.y, far[0][k] = z.x, far[1][k] = z.y;
                     } else {
                         near[0][k] = *reinterpret_cast<const uint32_t *>(at_near), far[0][k] = *reinterpret_cast<const uint32_t *>(at_far);
                     }
                 }
 #pragma unroll
                 for (int j = 0; j < L::kLoad; ++j) {
-                    uint32_t x[4], y[4];
+                    uint32_t x[4], z[4];
                     transpose_bytes(near[j], x);
-                    transpose_bytes(far[j], y);
+                    transpose_bytes(far[j], z);
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int b = 0; b < 2; ++b) {
-                            mma(acc[n][2 * (j0 + j)][b], x[0], x[1], y[0], y[1], w[n][b][0], w[n][b][1]);
-                            mma(acc[n][2 * (j0 + j) + 1][b], x[2], x[3], y[2], y[3], w[n][b][0], w[n][b][1]);
+                        for (int half = 0; half < 2; ++half) {
+                            float(&to)[4] = o[n][j0 + j];
+                            mma(acc[n][2 * (j0 + j) + half], x[2 * half], x[2 * half + 1], z[2 * half], z[2 * half + 1], w[n][0][0], w[n][0][1]);
+#pragma unroll
+                            for (int b = 3; b > 0; --b) {
+                                if (b == 3 && !deep) continue;
+                                int c[4] = {0, 0, 0, 0};
+                                mma(c, x[2 * half], x[2 * half + 1], z[2 * half], z[2 * half + 1], w[n][b][0], w[n][b][1]);
+                                const float of = b == 3 ? unit * 0x1p-30f : b == 2 ? unit * 0x1p-15f : unit;
+                                to[2 * half] = fmaf(float(c[0] * 256 + c[1]), of, to[2 * half]);
+                                to[2 * half + 1] = fmaf(float(c[2] * 256 + c[3]), of, to[2 * half + 1]);
+                            }
                         }
                 }
             }
             __syncwarp();  // every lane has read the values
             issue_values(i + S::kStages);
-            if (++since == kFlush) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n) flush(n, 1.f);
-                since = 0;
-            }
-        }
-        bad = __any_sync(~0u, bad);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            flush(n, 1.f);
-            if (bad)
-#pragma unroll
-                for (int j = 0; j < L::kQuads; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = CUDART_NAN_F;
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         __syncwarp();
+        bool some = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            flush(n, 1.f);
+            some = some || loss[n] != 0.f;
+        }
+        bad = __any_sync(~0u, bad);
+        some = __any_sync(~0u, some);
+        // Another pass, for the digits behind those of this one, where weights below kLow may have lost too much; E takes the same way. 56 digits a
+        // pass; what is below 2^-142 is left out.
+        if (pass || some) {
+            bool lost = some && pass < 2 && !bad;
+            if (pass == 0) {
+                bool small = false;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) loss[n] += __shfl_xor_sync(~0u, loss[n], d);
+#pragma unroll
+                    for (int j = 0; j < L::kQuads; ++j)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) small = small || fabsf(o[n][j][k]) * kLoss < 128.f * loss[n];
+                }
+                lost = __any_sync(~0u, small) && lost;
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int j = 0; j < L::kQuads; ++j)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        if (pass) o[n][j][k] += sums[(n * L::kQuads + j) * 4 + k];
+                        if (lost) sums[(n * L::kQuads + j) * 4 + k] = o[n][j][k];
+                    }
+            if (lost) {
+                ++pass;
+                unit *= 0x1p-56f;
+                ahead = look_up(0);
+                for (int i = 0; i < S::kStages - 1; ++i) {
+                    issue_keys(i);
+                    issue_values(i);
+                }
+                goto again;
+            }
+        }
+        if (bad)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int j = 0; j < L::kQuads; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = CUDART_NAN_F;
 
         // ---- the next segment's first stages are on their way while this one's warps are folded, in the stage that they leave free.
         // Outputs lie there as [group][quad][lane], four elements of head t each.
