@@ -338,10 +338,11 @@ int32_t jl_kv8_map(jl_ctx *ctx, jl_kv8_workspace *ws, const jl_kv8_map_args *arg
 
 /* Append. Row t of k and v is [kv_heads][head_dim], row strides in elements. With rope_cos / rope_sin (tables of jl_upload_rope,
  * [rope_rows][head_dim / 2]) pairs (2i, 2i + 1) of the keys are rotated by the angle of positions[t] first. Then, for each token
- * and head, scale = max |x| / 127 and code = x / scale rounded to the nearest (ties to even), as if computed without rounding
- * before; a row whose largest element is below 2^-100 is stored as zeros, one with an infinite or NaN element with a NaN scale and
- * codes 0, and so are the keys of a token whose position is outside the tables. Rows with a place outside the pages (such as
- * -1), and rows from *token_count on, are not stored. Places of one call have to differ. */
+ * and head, code = 127 x / max |x| rounded to the nearest (ties to even), as if computed without rounding before, and
+ * scale = max |x| / 127, rounded once (of a rotated key, whose largest element is binary32's, within 2^-22). A row whose largest
+ * element is below 2^-100 is stored as zeros, one with an infinite or NaN element with a NaN scale and codes 0, and so are the keys
+ * of a token whose position is outside the tables. Rows with a place outside the pages (such as -1), and rows from *token_count
+ * on, are not stored. Places of one call have to differ. */
 typedef struct {
     jl_kv8_pages pages;
     const void *k, *v;              /* [tokens], 16-byte aligned; strides multiples of 16 bytes and at least kv_heads * head_dim */

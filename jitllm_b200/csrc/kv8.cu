@@ -315,7 +315,10 @@ __global__ void __launch_bounds__(kAppendThreads, 9) append_kernel(const AppendP
             code[i] = __float_as_uint(y);
         }
         const bool again = lost || !(most >= 0x1p-99f && most < 0x1p125f) || border > 0.5f - (turned ? 0x1p-14f : 0x1p-16f);
+        // most / 127 with one rounding: the quotient by the rounded reciprocal, and its remainder, which is exact (Markstein 1990). The largest element
+        // of a rotated row is off by 2.5 of 2^-24 itself; that of the exact rotation took 23.1 us in place of 19.8 for 8191 rotated tokens.
         float scale = most * (1.f / 127.f);
+        scale = fmaf(fmaf(-127.f, scale, most), 1.f / 127.f, scale);
         // whether any lane of the row says so
         const unsigned says = __ballot_sync(~0u, again && here);
         if (says) {
