@@ -313,9 +313,10 @@ int32_t jl_kv8_workspace_free(jl_ctx *ctx, jl_kv8_workspace *ws);
 /* Block table and slot map. Sequence r holds held[r] tokens and gets added[r] more. Sequences are served in order: one whose
  * tokens need new blocks takes them from free_blocks, from *cursor on, and their ids follow the ids of its blocks in its row of
  * the table; the table's other entries are left as they are. A sequence is refused (nothing of it changes, its tokens get
- * position and place -1) if held or added is negative, if it would grow beyond blocks_per_slot blocks or 2^31 - 1 tokens, if its tokens do not all
- * lie within `capacity`, or if the blocks it needs, together with those that the sequences before it need (refused for lack of
- * blocks or not), are more than there are.
+ * position and place -1) if held or added is negative, if it would grow beyond blocks_per_slot blocks or 2^31 - 1 tokens, if the
+ * tokens of the sequences up to and with it are more than `capacity` (behind one that does not fit all are refused, those without
+ * new tokens too), or if the blocks it needs, together with those that the sequences before it need (refused for lack of blocks
+ * or not), are more than there are (one that needs none is not refused for that).
  * New tokens are numbered through, sequence after sequence: token offsets[r] + i is sequence r's token at position held[r] + i
  * and belongs at place block * block_tokens + position % block_tokens of the pages (-1 where the table holds no block >= 0).
  * Entries of the token arrays from the last token on are left as they are. */
