@@ -14,6 +14,16 @@ from . import _lib
 from .api import Device, GGMLType, IllegalStateError
 
 
+def _struct(kind, *values):
+    """The argument structure. ctypes would cut a number that its field has no room for."""
+    for (name, field), value in zip(kind._fields_, values):
+        if field in (C.c_int32, C.c_int64, C.c_void_p) and value is not None:
+            bits = 8 * C.sizeof(field)
+            if not (0 if field is C.c_void_p else -(1 << bits - 1)) <= value < 1 << (bits if field is C.c_void_p else bits - 1):
+                raise ValueError(f"{name} = {value} does not fit into {bits} bits")
+    return kind(*values)
+
+
 class Kv8Workspace:
     """Partial results and arrival counters of jl_kv8_map and jl_kv8_attention. Calls with one workspace must not overlap on
     the GPU: one for each stream (or captured graph) that runs beside others. Closed with the device at the latest: keep it
@@ -52,8 +62,8 @@ class Kv8Pages:
                  kvHeads: int, headSize: int, blockStride: Optional[int] = None, scaleStride: Optional[int] = None):
         self.dev = dev
         rows = kvHeads * blockSizeTokens
-        self.struct = _lib.JlKv8Pages(
-            k, v, kScale, vScale, rows * headSize if blockStride is None else blockStride,
+        self.struct = _struct(
+            _lib.JlKv8Pages, k, v, kScale, vScale, rows * headSize if blockStride is None else blockStride,
             rows if scaleStride is None else scaleStride, blocks, blockSizeTokens, kvHeads, headSize)
 
     def bytesPerBlock(self) -> int:
@@ -87,8 +97,8 @@ class Kv8Map(_Call):
     def __init__(self, workspace: Kv8Workspace, *, held: int, added: int, sequences: int, blockTable: int, blocksPerSlot: int,
                  blockSizeTokens: int, freeBlocks: int, freeCount: int, cursor: int, cursorOut: int, lengths: int,
                  slotMap: int, capacity: int, result: int, offsets: int = 0, tokenSlots: int = 0, positions: int = 0):
-        super().__init__(workspace.dev, "jl_kv8_map", _lib.JlKv8MapArgs(
-            held, added, freeBlocks, cursor, cursorOut, blockTable, lengths, offsets, tokenSlots, positions, slotMap, result,
+        super().__init__(workspace.dev, "jl_kv8_map", _struct(
+            _lib.JlKv8MapArgs, held, added, freeBlocks, cursor, cursorOut, blockTable, lengths, offsets, tokenSlots, positions, slotMap, result,
             sequences, blocksPerSlot, blockSizeTokens, freeCount, capacity), workspace)
 
 
@@ -100,8 +110,8 @@ class Kv8Append(_Call):
                  keyStride: Optional[int] = None, valueStride: Optional[int] = None, positions: int = 0, ropeCos: int = 0,
                  ropeSin: int = 0, ropeRows: int = 0, tokenCount: int = 0):
         row = pages.struct.kv_heads * pages.struct.head_dim
-        super().__init__(pages.dev, "jl_kv8_append", _lib.JlKv8AppendArgs(
-            pages.struct, k, v, row if keyStride is None else keyStride, row if valueStride is None else valueStride, slotMap,
+        super().__init__(pages.dev, "jl_kv8_append", _struct(
+            _lib.JlKv8AppendArgs, pages.struct, k, v, row if keyStride is None else keyStride, row if valueStride is None else valueStride, slotMap,
             positions, ropeCos, ropeSin, tokenCount, tokens, ropeRows, int(ggml_type)))
 
 
@@ -115,7 +125,7 @@ class Kv8Attention(_Call):
                  scale: Optional[float] = None, ropeCos: int = 0, ropeSin: int = 0, ropeRows: int = 0, tokenCount: int = 0):
         d = pages.struct.head_dim
         row = heads * d
-        super().__init__(pages.dev, "jl_kv8_attention", _lib.JlKv8AttentionArgs(
-            pages.struct, q, out, lse, row if queryStride is None else queryStride, row if outStride is None else outStride,
+        super().__init__(pages.dev, "jl_kv8_attention", _struct(
+            _lib.JlKv8AttentionArgs, pages.struct, q, out, lse, row if queryStride is None else queryStride, row if outStride is None else outStride,
             blockTable, kvSlots, positions, ropeCos, ropeSin, tokenCount, rows, heads, slots, blocksPerSlot, window, ropeRows,
             int(ggml_type), d ** -0.5 if scale is None else scale), workspace)
