@@ -303,7 +303,7 @@ typedef struct {
     int32_t blocks, block_tokens, kv_heads, head_dim;
 } jl_kv8_pages;
 
-/* Device memory that jl_kv8_map and jl_kv8_attention keep their partial results and arrival counters in: about 5 MB, made once, not while a stream is being captured.
+/* Device memory that jl_kv8_map and jl_kv8_attention keep their partial results and arrival counters in: about 5.5 MB, made once, not while a stream is being captured.
  * Calls with one workspace must not overlap on the GPU: one workspace for each stream (or captured graph) that runs beside
  * others. Calls of any shape may follow one another. Free it when no call with it is under way and no graph holds one. */
 typedef struct jl_kv8_workspace jl_kv8_workspace;
@@ -364,7 +364,8 @@ int32_t jl_kv8_append(jl_ctx *ctx, const jl_kv8_append_args *args, void *stream)
  * weight. A row that attends to nothing (position -1, a sequence outside 0..slots - 1) gets zeros and lse -inf; rows from
  * *token_count on are left as they are. A NaN scale, query or key makes NaN of the outputs that it has weight in. Scores and sums are
  * binary32 (scale times a query times codes has to be finite in it); a token's softmax weight times its scale is taken to 2^-18 of
- * itself where it is within 2^-39 of the largest of its sequence, and smaller ones lose 2^-13 of an output together at most. */
+ * itself where it is within 2^-41 of the largest of its sequence; smaller ones lose 2^-13 of an output together at most, and those
+ * below 2^-150 of the largest count as 0. */
 typedef struct {
     jl_kv8_pages pages;
     const void *q;                  /* [rows], 16-byte aligned, row stride in elements a multiple of 16 bytes */

@@ -27,8 +27,9 @@ void kv8_division(int divisor, uint64_t *divide, int *shift);
 // Lets a kernel have so many bytes of dynamic shared memory on the current device; `configured` has a bit for each device.
 cudaError_t kv8_allow_shared(const void *kernel, int bytes, std::atomic<uint64_t> &configured);
 
-// One launch; programmatic: the grid may be set up while the kernel ahead of it in the stream still runs. Each of these kernels lets
-// its successor do so as soon as it starts, and touches no memory before everything ahead of it is over (pdl_wait).
+// One launch; programmatic: the grid may be set up while the kernel ahead of it in the stream still runs. Map and append let their
+// successor do so as soon as they start, the attention when its CTAs are through their last loops; each touches no memory before
+// everything ahead of it is over (pdl_wait).
 template <typename P>
 cudaError_t kv8_launch(void (*kernel)(const P), unsigned grid, unsigned threads, size_t shared, cudaStream_t stream, bool programmatic, const P &params) {
     cudaLaunchConfig_t cfg = {};

@@ -1,38 +1,39 @@
 // Attention of single tokens over the 8-bit paged key/value cache.
 //
-// Work. A unit is one row and four or eight query heads of one KV head; its tokens are cut into tiles of 64. The tiles of all units
-// form one line (rows in order, then heads, then tokens), of which every CTA of a grid that fits the GPU takes an equal piece. The
+// Work. A unit is one row and four or eight query heads of one KV head; its tokens are cut into tiles of 128 (of 64 with head sizes above
+// 128). The tiles of all units form one line (rows in order, then heads, then tokens), of which every CTA of a grid that fits the GPU takes an equal piece. The
 // lengths are on the device, so each CTA works the line out for itself from the rows' positions. A unit that lies within a piece is
 // finished there; the parts of one that is cut are left in the workspace, and the CTA that arrives last at the unit's counter joins
 // them in order, so results do not hang on who arrives when.
 //
 // Mathematics. s = scale * ks_j * (q . kc_j), weights p_j = 2^(s_j log2 e - m) with a running reference m, and
 // out = sum p_j vs_j vc_j / sum p_j. Both products are of integers: a query is rounded to 31 bits of its head's largest element and
-// cut into four signed bytes (a balanced radix of 256), and so is the whole part of the weight w_j = 2^(s_j log2 e - E) vs_j, with a power
-// of two E that moves on when a weight would pass 2^30. Its fraction has four bytes more, 15 bits in each two. Two bytes of four heads are
-// the columns of an mma.m16n8k32 (int8, sums in int32), whose rows are tokens (keys) or elements (values): the codes go in as they
-// are, without a conversion (values after a transpose of four by four bytes), and a step's sums are exact. E follows the weights with
-// the scale, so scales of values may differ by any factor between tokens; m and E are whole numbers, so that moving them on rounds nothing.
+// cut into four signed bytes (a balanced radix of 256), and the weight w_j = 2^(s_j log2 e - E) vs_j is cut into eight of them, in units of
+// 2^-32, with a power of two E that moves on when a weight would pass 2^30. Two bytes of four heads are the columns of an mma.m16n8k32
+// (int8, sums in int32), whose rows are tokens (keys) or elements (values): the codes go in as they are, without a conversion
+// (values after a transpose of four by four bytes), and a step's sums are exact. E follows the weights with the scale, so scales of
+// values may differ by any factor between tokens; m and E are whole numbers, so that moving them on rounds nothing.
 //
 // What small weights keep. A token far above the others says nothing about an element where its code is 0; that is made up of the
 // others, whose weights must not drown in the digits of the large one. A warp's largest weight times scale is above 2^26, so one within
-// 2^-39 of it (27 nats) is cut off by less than 2^-18 of itself. What the smaller ones lose is added up, and where it could be more than
-// 2^-13 of an output, the warp goes over its tokens again for the digits behind those. Whole numbers alone, which lose a weight
-// of 2^-28 of the largest, took (us) 184 for 16 rows at 32000, 11.2 for one row at 3901, 12.6 for 32 rows at 512, 18.2 for 64 rows with a window
-// of 1000; these take 172, 11.6, 13.7 and 20.8. A second pass doubles them: 66 us in place of 49 for 16 rows at 2000 of head size 256 and scores of 3 nats.
+// 2^-41 of it (28 nats) is off by 2^-18 of itself at most. What the smaller ones lose is added up, and where it could be more than 2^-13 of an
+// output, the warp goes over its tokens again for the digits behind those (exponentials end at 2^-126, 150 octaves below). Four bytes alone, which lose a weight of 2^-28 of the
+// largest, took (us) 191 for 16 rows at 32000, 11.3 for one row at 3901, 12.9 for 32 rows at 512, 18.9 for 64 rows with a window of 1000; these take
+// 207, 11.5, 13.6 and 21.6. A second pass doubles a warp's time; with scores of 3 nats some warp of a large grid has one in one call of three or so.
 //
-// What bounds it (kernel alone, back to back; copy rate 6.46 TB/s). 16 rows at 32000 tokens of 8 KV heads of 128, 1.08 GB: 186 us, 5.8 TB/s; with
-// equal pieces the SMs are through between 0.85 and 1.15 of the mean, since they do not get their data at one rate. 64 rows with a
-// window of 1000 of 8 KV heads of 64, 70 MB: 18.8 us, 3.7 TB/s; a step of 32 tokens costs about 370 instructions whatever the head
-// size. 32 rows at 512 of 8 of 128, 31 MB: 12.7 us; one row at 3901, 8 MB: 11.1 us; one at 57: 4.6 us. These are chains: lengths, blocks, keys,
-// two to four steps of 0.8 us, 0.6 us to fold the warps, 2 us to publish a part and hear who is last, 1.5 us to join. Dealing the
-// last quarter of a long line out in chunks was slower (a change of units costs more than what the SMs differ by), and so were warps
-// of their own for units, next segments entered ahead, and a smaller kernel made of loops.
+// What bounds it (back to back on three sets of inputs in turn; copy rate 6.46 TB/s). 16 rows at 32000 tokens of 8 KV heads of 128, 1.08 GB: 207 us, 5.2
+// TB/s, after a second at the power limit of the card (1000 W, 1.5 GHz), 192 us in front of it: the bytes, and the energy of what is computed.
+// 64 rows with a window of 1000 of 8 KV heads of 64, 70 MB: 21.6 us, 3.2 TB/s: instructions, issued in 0.58 of the cycles by 13 warps of an SM. 32
+// rows at 512 of 8 of 128, 31 MB: 13.6 us; one row at 3901, 8 MB: 11.5 us; one at 57: 5.0 us. These are chains: lengths, blocks, keys, one to five steps
+// of about 1 us, 0.6 us to fold the warps, 2 us to publish a part and hear who is last, 1.5 us to join. Dealing the last quarter of a long
+// line out in chunks was slower (a change of units costs more than what the SMs differ by), and so were warps of their own for units,
+// next segments entered ahead, and a smaller kernel made of loops.
 #include <cuda_fp16.h>
 #include <math_constants.h>
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kv8.cuh"
@@ -42,7 +43,7 @@ namespace {
 
 constexpr int kStep = 32;                // tokens that a warp takes at a time
 constexpr uint32_t kLongQuota = 8;       // tiles for each CTA from which on lines are cut without regard to units. 4 / 8 / 16: 64 rows with a
-                                         // window of 1000 24.7 / 20.5 / 20.5 us, 8 rows at 2000 of 8 groups of 8 heads 23.6 / 23.0 / 25.4
+                                         // window of 1000 27.5 / 21.6 / 21.6 us, 8 rows at 2000 of 8 groups of 8 heads 22.6 / 20.6 / 20.6
 constexpr int kRowsPerLane = 4;          // of up to 128 rows, short lines of which are cut by units
 constexpr int kMostSms = 160, kMostCtas = 4 * kMostSms;
 constexpr uint32_t kGroup = 32;          // parts that are joined at once
@@ -51,7 +52,7 @@ static_assert(kMostCtas <= int(kGroup * kGroup));
 constexpr int kFlush = 2048;             // steps after which sums of 2^14 a token could pass 2^30
 constexpr float kNothing = -3e38f;       // m and E before there is a token
 constexpr float kHeadroom = 26.f;        // E moves on so that weights are below 2^27, and again when one passes 1.5e9 or could pass 2^30
-constexpr float kDeep = 0x1p2f, kLow = kDeep * 0x1p-15f;  // weights that are off by 2^-18 of themselves at most with 15 bits of their fraction, and with 30
+constexpr float kDeep = 0x1p1f, kLow = 0x1p-15f;  // weights that are off by 2^-18 of themselves at most with six bytes, and with eight
 constexpr float kLoss = 0x1p-13f;        // of an output, that weights below the second may lose
 constexpr float kMagic = 12582912.f;     // 1.5 * 2^23: a sum's low bits are those of the whole number, to the nearest
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
@@ -84,19 +85,20 @@ struct Layout {
     }
 };
 
-// NT groups of four query heads have HD / 2 * NT accumulators. What these and the stages leave room for, with both sides measured (us):
-// head size 128, 2 CTAs of 3 stages and 3 CTAs of 2: 13.3 / 14.9 (32 rows at 512 of 8 KV heads), 18.0 / 20.6 (1 row at 20000); 64 with one group,
-// 4 CTAs of 3 and 3 of 4: 20.5 / 24.4 (64 rows, a window of 1000), 9.1 / 9.3 (1 row at 4000), with two groups, 2 of 6 and 3 of 4: 12.5 / 16.4 (8
-// rows at 2000 of 4 KV heads); 96, 3 of 2 and 2 of 4: 17.2 / 18.3 (16 rows at 2000), two groups 17.0 / 13.6; 256, 2 of 3 and 3 of 2: 19.0 / 20.5.
+// NT groups of four query heads have 3 / 8 * HD * NT accumulators. What these and the stages leave room for, with both sides measured (us): head
+// size 128, 2 CTAs of 3 stages and 3 CTAs of 2: 13.6 / 15.8 (32 rows at 512 of 8 KV heads), 18.1 / 20.8 (1 row at 20000), 192 / 192 (16 rows at 32000), but
+// 24.8 / 20.1 (128 rows at 100); 64 with one group, 4 CTAs of 3 and 3 of 4: 21.6 / 25.0 (64 rows, a window of 1000), but 124 / 117 (16 rows at 32000), with
+// two groups, 2 of 6 and 3 of 4: 13.3 / 15.2 (8 rows at 2000 of 4 KV heads); 96, 3 of 2 and 2 of 4: 17.9 / 18.6 (16 rows at 2000); 192, 3 of 2 and 2 of
+// 3: 33.3 / 36.8 (16 rows at 2000), 84 / 89 (at 8000), but 20.5 / 18.0 (1 row at 5000); 256, 2 of 3 and 2 of 2: 49.3 / 52.7 (16 rows at 2000).
 template <int HD, int NT>
 struct Shape {
     static constexpr int kWarps = HD <= 128 ? 4 : 2, kThreads = 32 * kWarps;
     static constexpr int kTile = kStep * kWarps;  // tokens of a tile
-    static constexpr int kStages = HD == 64 ? (NT == 1 ? 3 : 6) : HD == 96 ? (NT == 1 ? 2 : 4) : 3;
+    static constexpr int kStages = HD == 64 ? (NT == 1 ? 3 : 6) : HD == 96 || HD == 192 ? 2 : 3;
     static constexpr int kRing = kStages * Layout<HD>::kStage, kBytes = kWarps * kRing;
     static constexpr int kHeads = 4 * NT, kPartFloats = kHeads * (HD + 3);
     static constexpr int kShare = HD / 16 / kWarps + (HD / 16 % kWarps != 0);  // words of the queries that a warp prepares
-    static constexpr int kResident = NT == 1 && HD == 64 ? 4 : NT == 1 && HD == 96 ? 3 : 2;  // CTAs per SM
+    static constexpr int kResident = NT == 1 && HD == 64 ? 4 : HD == 96 || HD == 192 ? 3 : 2;  // CTAs per SM
     static_assert(kResident * kMostSms <= kMostCtas);
     static_assert(Layout<HD>::kStage >= kHeads * HD * 4);  // a stage also holds a warp's outputs
     static_assert(kResident * (kBytes + NT * HD * 16 + kWarps * kShare * (NT * 256 + 64) + 128 * kHeads + 1024) <= 228 * 1024);
@@ -358,7 +360,9 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
         code_at = good ? block * a.pages.block_stride + in_block * HD : -1;
         scale_at = good ? block * a.pages.scale_stride + in_block : -1;
     };
-    // Codes that no other CTA wants are the first to leave L2 (16 rows at 32000: 187 / 194 us with / without, head size 64 97 / 113).
+    // Codes that no CTA reads for other heads of its unit's are the first to leave L2: with and without, 16 rows at 32000 192 / 197 us, 64 rows with a
+    // window of 1000 21.6 / 22.8, 16 rows at 8000 of head size 192 84 / 89. Rows that read the same blocks find most of them there all the same: 32 rows of
+    // one sequence of 4000 tokens 50.5 / 50.4, of 16000 168 / 157, 128 rows of 4000 166 / 166, a third of the blocks in common 50.5 / 51.0.
     const uint64_t policy = p.head_tiles == 1 ? policy_evict_first() : policy_normal();
     // Keys, scales and mask of step i, and its values, as groups of copies of their own.
     auto copy_rows = [&](int i, const int8_t *pages, uint32_t stage) {
@@ -566,13 +570,12 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
         // ---- one pass over this warp's tokens: lane (g, t) has tokens g, g + 8, g + 16, g + 24 of a step, heads 4 n + t, elements of
         // column g. The four tokens of g are bytes of one word of weights, and so are those of t and of t + 4 in a word of values.
         float m[NT], e[NT], l[NT], o[NT][L::kQuads][4];
-        int acc[NT][2 * L::kQuads][4];  // elements 2 i and 2 i + 1 of a word; bytes 3 and 2 of the weights
+        int acc[NT][2 * L::kQuads][4];  // elements 2 i and 2 i + 1 of a word; bytes 7 and 6 of the weights
         float loss[NT];                 // of weights below kLow
         bool bad = false;               // a value's scale was no number
         int since, pass = 0;            // steps in `acc`; passes over the tokens in front of this one
         float unit = 1.f;               // of this pass's weights, next to 2^E
         volatile float sums[NT * L::kQuads * 4];  // of the passes in front
-        auto rest = [](float x) { return fmaf(x, 0x1p15f, kMagic - fmaf(x, 0x1p15f, kMagic)); };  // what a fraction's next 15 bits leave: exact
         // o = (o + acc) keep, acc = 0; the other bytes' products are in `o` already
         auto flush = [&](int n, float keep) {
 #pragma unroll
@@ -580,9 +583,10 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     int(&c)[4] = acc[n][j];
-                    const float x = since <= 8 ? float(c[2 * k] * 256 + c[2 * k + 1]) : fmaf(float(c[2 * k]), 256.f, float(c[2 * k + 1]));  // below 2^22 each: two fit one number
                     float &y = o[n][j / 2][2 * (j & 1) + k];
-                    y = fmaf(x, 65536.f * unit, y) * keep;
+                    // below 2^22 each: two fit one number
+                    const float x = since <= 8 ? float(c[2 * k] * 256 + c[2 * k + 1]) : fmaf(float(c[2 * k]), 256.f, float(c[2 * k + 1]));
+                    y = fmaf(x, unit * 0x1p16f, y) * keep;
                     c[2 * k] = c[2 * k + 1] = 0;
                 }
         };
@@ -678,63 +682,53 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
                 for (int k = 0; k < 4; ++k) l[n] += exp2_approx(x[k] - m[n]);
                 for (int times = 0; times < pass; ++times)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) y[n][k] = rest(rest(y[n][k] - float(__float2int_rn(y[n][k])))) * 0x1p26f;
+                    for (int k = 0; k < 4; ++k) {
+                        const float z = y[n][k] * 0x1p32f;
+                        y[n][k] = (z - __ll2float_rn(__float2ll_rn(z))) * 0x1p26f;  // exact
+                    }
 #pragma unroll
                 for (int k = 0; k < 4; ++k) least = fminf(least, fabsf(y[n][k]));
             }
-            // The fraction's second 15 bits only where a weight is below 4, or always: head size 64, 64 rows with a window of 1000 20.8 / 22.1 us; 128, 16
-            // rows at 32000 187 / 172 and 32 rows at 512 13.6 / 13.9, with scores of twice the size 206 / 178 and 15.0 / 14.2.
-            const bool deep = HD > 64 || __any_sync(~0u, least < kDeep);
+            // The last two bytes only where a weight is below 2: 16 rows at 32000 207 us, 214 with them always; 32 rows at 512 13.6 / 13.9; 64 rows
+            // with a window of 1000 21.6 / 22.3.
+            const bool deep = __any_sync(~0u, least < kDeep);
             if (moved || since == kFlush) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) flush(n, keep[n]);
                 since = 0;
             }
             ++since;
-            // The columns, as of the queries: of whole numbers (two pairs of bytes), of their fractions' first 15 bits, and of the next 15 where they
-            // count. Lane (g, t) has the bytes of head t and tokens g; column g is of head g / 2; groups of tokens t and t + 4.
+            // Weights as eight signed bytes, in units of 2^-32; pairs of them are columns, as of the queries. Lane (g, t) has the bytes of head t and
+            // tokens g; column g is of head g / 2; groups of tokens t and t + 4.
             uint32_t w[NT][4][2];
-            auto columns = [&](const uint32_t (&bytes)[4], int n, int high, int b) {
-#pragma unroll
-                for (int far = 0; far < 2; ++far) {
-                    const int from = (t + 4 * far) * 4 + (g >> 1);
-                    const uint32_t even = __shfl_sync(~0u, bytes[high], from), odd = __shfl_sync(~0u, bytes[high - 1], from);
-                    w[n][b][far] = g & 1 ? odd : even;
-                }
-            };
-            auto fraction_columns = [&](const float (&x)[4], int n, int b) {
-                uint32_t sums[4], digit[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) sums[k] = __float_as_uint(fmaf(x[k], 0x1p15f, kMagic + 128.f));  // of two signed bytes, the second and 128
-                transpose_bytes(sums, digit);
-                digit[0] ^= 0x80808080u;
-                columns(digit, n, 1, b);
-            };
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                uint32_t bytes[4], digit[4];
+                uint32_t low[4], high[4], digit[4];
+                auto columns = [&](int pair, int upper) {
+#pragma unroll
+                    for (int far = 0; far < 2; ++far) {
+                        const int from = (t + 4 * far) * 4 + (g >> 1);
+                        const uint32_t even = __shfl_sync(~0u, digit[upper], from), odd = __shfl_sync(~0u, digit[upper - 1], from);
+                        w[n][pair][far] = g & 1 ? odd : even;
+                    }
+                };
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const int whole = __float2int_rn(y[n][k]);  // NaN becomes 0
-                    y[n][k] -= float(whole);                    // exact; 0 from 2^23 on
-                    bytes[k] = signed_bytes(whole);
+                    const uint64_t bytes = (uint64_t(__float2ll_rn(y[n][k] * 0x1p32f)) + 0x0080808080808080u) ^ 0x0080808080808080u;
+                    low[k] = uint32_t(bytes), high[k] = uint32_t(bytes >> 32);
                 }
-                transpose_bytes(bytes, digit);
-                columns(digit, n, 3, 0);
-                columns(digit, n, 1, 1);
-                fraction_columns(y[n], n, 2);
+                transpose_bytes(high, digit);
+                columns(0, 3);
+                columns(1, 1);
+                transpose_bytes(low, digit);
+                columns(2, 3);
+                if (deep) columns(3, 1);
             }
-            if (deep) {
+            if (deep && __any_sync(~0u, least < kLow)) {
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        // of the fraction's bits; where there is a whole number in front of them the loss is less
-                        loss[n] += fabsf(y[n][k]) < kLow ? fminf(fabsf(y[n][k]), 0x1p-31f) : 0.f;
-                        y[n][k] = rest(y[n][k]);
-                    }
-                    fraction_columns(y[n], n, 3);
-                }
+                    for (int k = 0; k < 4; ++k) loss[n] += fabsf(y[n][k]) < kLow ? fminf(fabsf(y[n][k]), 0x1p-33f) : 0.f;
             }
 
             __syncwarp();  // every lane has read keys and scales
@@ -742,43 +736,46 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
             asm volatile("cp.async.wait_group %0;" ::"n"(2 * S::kStages - 1) : "memory");
             __syncwarp();
             // values: of a word of column g, elements 0 and 1 are rows g and g + 8 of one product, 2 and 3 of the next
+            auto multiply = [&](auto pairs) {
 #pragma unroll
-            for (int j0 = 0; j0 < L::kQuads; j0 += L::kLoad) {
-                uint32_t near[L::kLoad][4], far[L::kLoad][4];  // tokens t + 8 k, t + 4 + 8 k
-                const int el = L::value_element(g, j0);
+                for (int j0 = 0; j0 < L::kQuads; j0 += L::kLoad) {
+                    uint32_t near[L::kLoad][4], far[L::kLoad][4];  // tokens t + 8 k, t + 4 + 8 k
+                    const int el = L::value_element(g, j0);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const unsigned char *at_near = stage + L::kValues + L::piece(t + 8 * k, el >> 4) + (el & 15), *at_far = stage + L::kValues + L::piece(t + 4 + 8 * k, el >> 4) + (el & 15);
-                    if constexpr (L::kLoad == 2) {
-                        const uint2 x = *reinterpret_cast<const uint2 *>(at_near), z = *reinterpret_cast<const uint2 *>(at_far);
-                        near[0][k] = x.x, near[1][k] = x.y, far[0][k] = z.x, far[1][k] = z.y;
-                    } else {
-                        near[0][k] = *reinterpret_cast<const uint32_t *>(at_near), far[0][k] = *reinterpret_cast<const uint32_t *>(at_far);
+                    for (int k = 0; k < 4; ++k) {
+                        const unsigned char *at_near = stage + L::kValues + L::piece(t + 8 * k, el >> 4) + (el & 15), *at_far = stage + L::kValues + L::piece(t + 4 + 8 * k, el >> 4) + (el & 15);
+                        if constexpr (L::kLoad == 2) {
+                            const uint2 x = *reinterpret_cast<const uint2 *>(at_near), z = *reinterpret_cast<const uint2 *>(at_far);
+                            near[0][k] = x.x, near[1][k] = x.y, far[0][k] = z.x, far[1][k] = z.y;
+                        } else {
+                            near[0][k] = *reinterpret_cast<const uint32_t *>(at_near), far[0][k] = *reinterpret_cast<const uint32_t *>(at_far);
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < L::kLoad; ++j) {
+                        uint32_t x[4], z[4];
+                        transpose_bytes(near[j], x);
+                        transpose_bytes(far[j], z);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) {
+                                float(&to)[4] = o[n][j0 + j];
+#pragma unroll
+                                for (int b = decltype(pairs)::value - 1; b > 0; --b) {
+                                    int c[4] = {0, 0, 0, 0};
+                                    mma(c, x[2 * half], x[2 * half + 1], z[2 * half], z[2 * half + 1], w[n][b][0], w[n][b][1]);
+                                    const float of = unit * (b == 3 ? 0x1p-32f : b == 2 ? 0x1p-16f : 1.f);
+                                    to[2 * half] = fmaf(float(c[0] * 256 + c[1]), of, to[2 * half]);
+                                    to[2 * half + 1] = fmaf(float(c[2] * 256 + c[3]), of, to[2 * half + 1]);
+                                }
+                                mma(acc[n][2 * (j0 + j) + half], x[2 * half], x[2 * half + 1], z[2 * half], z[2 * half + 1], w[n][0][0], w[n][0][1]);
+                            }
                     }
                 }
-#pragma unroll
-                for (int j = 0; j < L::kLoad; ++j) {
-                    uint32_t x[4], z[4];
-                    transpose_bytes(near[j], x);
-                    transpose_bytes(far[j], z);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            float(&to)[4] = o[n][j0 + j];
-                            mma(acc[n][2 * (j0 + j) + half], x[2 * half], x[2 * half + 1], z[2 * half], z[2 * half + 1], w[n][0][0], w[n][0][1]);
-#pragma unroll
-                            for (int b = 3; b > 0; --b) {
-                                if (b == 3 && !deep) continue;
-                                int c[4] = {0, 0, 0, 0};
-                                mma(c, x[2 * half], x[2 * half + 1], z[2 * half], z[2 * half + 1], w[n][b][0], w[n][b][1]);
-                                const float of = b == 3 ? unit * 0x1p-30f : b == 2 ? unit * 0x1p-15f : unit;
-                                to[2 * half] = fmaf(float(c[0] * 256 + c[1]), of, to[2 * half]);
-                                to[2 * half + 1] = fmaf(float(c[2] * 256 + c[3]), of, to[2 * half + 1]);
-                            }
-                        }
-                }
-            }
+            };
+            if (deep) multiply(std::integral_constant<int, 4>());
+            else multiply(std::integral_constant<int, 3>());
             __syncwarp();  // every lane has read the values
             issue_values(i + S::kStages);
         }
@@ -792,8 +789,8 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
         }
         bad = __any_sync(~0u, bad);
         some = __any_sync(~0u, some);
-        // Another pass, for the digits behind those of this one, where weights below kLow may have lost too much; E takes the same way. 56 digits a
-        // pass; what is below 2^-142 is left out.
+        // Another pass, for the digits behind those of this one, where weights below kLow may have lost too much; E takes the same way. 58 binary
+        // digits a pass; what is below 2^-148 is left out.
         if (pass || some) {
             bool lost = some && pass < 2 && !bad;
             if (pass == 0) {
@@ -820,7 +817,7 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
                     }
             if (lost) {
                 ++pass;
-                unit *= 0x1p-56f;
+                unit *= 0x1p-58f;
                 ahead = look_up(0);
                 for (int i = 0; i < S::kStages - 1; ++i) {
                     issue_keys(i);
@@ -1004,13 +1001,14 @@ cudaError_t launch(Params &p, const Kv8Scratch &s, const Kv8Launch &l) {
 
 template <int HD>
 cudaError_t launch_head(Params &p, const Kv8Scratch &s, const Kv8Launch &l) {
-    // Blocks of multiples of 16 tokens: one lookup for sixteen rows instead of one for each. One row at 3901 11.3 / 11.8 us, 32 rows at 512
-    // 12.9 / 14.6 (16 rows at 32000, bound by memory, 193 / 183 before codes left L2 first).
+    // Blocks of multiples of 16 tokens: one lookup for sixteen rows instead of one for each. One row at 3901 11.5 / 12.0 us, 32 rows at 512
+    // 13.6 / 15.5, 16 rows at 32000 192 / 227.
     const bool paged16 = p.a.pages.block_tokens % 16 == 0;
     // More than four query heads of a KV head: eight to a unit, or four, whose CTAs then read a token's keys and values twice (from L2 the
-    // second time). Head size 128, eight heads, four and eight to a unit (us): 8 rows at 2000 of 8 KV heads 21.2 / 24.2, at 16000 76 / 88, 1 row at
-    // 100000 of one 21.1 / 26.3; but 32 rows at 300 20.6 / 17.4, where units are many. Head size 64: 16 rows at 16000 of 4 KV heads 53.3 / 50.2.
-    if constexpr (HD <= 128)
+    // second time). Eight heads, four and eight to a unit (us): head size 128, 8 rows at 2000 of 8 KV heads 20.6 / 21.6, 1 row at 100000 of one
+    // 21.8 / 25.5, at 16000 92 / 80; where units are many, 32 rows at 300 22.4 / 16.7, 24 rows at 800 27.8 / 25.4, 64 rows at 1500 82 / 92. Head size 64: 16
+    // rows at 16000 of 4 KV heads 64 / 56. Head size 96: 24 rows at 300 11.2 / 14.0, 64 rows at 1000 48 / 64, 32 rows at 2000 43 / 49, but 32 rows at 300 18.1 / 14.4.
+    if constexpr (HD == 64 || HD == 128)
         if (p.group > 4 && (HD == 64 || int64_t(p.a.rows) * p.a.pages.kv_heads >= l.sm_count)) return paged16 ? launch<HD, 2, true>(p, s, l) : launch<HD, 2, false>(p, s, l);
     return paged16 ? launch<HD, 1, true>(p, s, l) : launch<HD, 1, false>(p, s, l);
 }
@@ -1025,7 +1023,7 @@ constexpr size_t kPartsPerSm = size_t(kSlots) * Shape<HD, NT>::kResident *Shape<
 cudaError_t kv8_scratch_create(Kv8Scratch *s, int sm_count) {
     if (sm_count > kMostSms) return cudaErrorInvalidValue;  // more CTAs than there are counters, or than a join has room for
     // for the CTAs of the largest grid, of the largest kind
-    const size_t parts = std::max({kPartsPerSm<64, 1>, kPartsPerSm<64, 2>, kPartsPerSm<96, 1>, kPartsPerSm<96, 2>, kPartsPerSm<128, 1>, kPartsPerSm<128, 2>, kPartsPerSm<192, 1>,
+    const size_t parts = std::max({kPartsPerSm<64, 1>, kPartsPerSm<64, 2>, kPartsPerSm<96, 1>, kPartsPerSm<128, 1>, kPartsPerSm<128, 2>, kPartsPerSm<192, 1>,
                                    kPartsPerSm<256, 1>});
     cudaError_t e = cudaMalloc(&s->memory, kKv8CounterBytes + size_t(sm_count) * parts);
     if (e == cudaSuccess) e = cudaMemset(s->memory, 0, kKv8CounterBytes);

@@ -20,7 +20,8 @@ def ws(dev):
 
 
 def _terms(a, r, h):
-    """Row r, query head h in 64 bits: scores [tokens], outputs and the sums of their terms' magnitudes [size]."""
+    """Row r, query head h in 64 bits: scores [tokens], outputs and the sums of their terms' magnitudes [size]; and of those terms whose weight
+    times scale is below 2^-150 of the largest one: the largest is 2^26 units or more, and exponentials end at 2^-126 units."""
     codes, scales = a.p.host()
     n = int(a.positions[r]) + 1
     j = np.arange(n)
@@ -31,18 +32,19 @@ def _terms(a, r, h):
     s = k @ a.q[r, h * a.d:(h + 1) * a.d].astype(np.float64) * a.scale
     p = np.exp(s - s.max())
     p /= p.sum()
-    return s, p @ v, p @ np.abs(v)
+    weight = p * scales[1, b, kv, j % a.block]
+    return s, p @ v, p @ np.abs(v), np.where(weight < 2.0 ** -150 * weight.max(), p, 0) @ np.abs(v)
 
 
 def _tolerance(s, v_octaves, steps):
     """Of an output, relative to the sum of its terms' magnitudes. With X the largest |score| and G the widest distance of two
     scores in octaves (v_octaves: of two scales of values; 31: the room that weights have above), a weight is off by the score's five
     roundings and the subtraction's (2^-24 (5 X + G + v_octaves + 31) ln 2), the exponential (2^-22), the product with its scale (2^-24) and
-    the digits that it is cut into (2^-18); the same but the last two again in the denominator. Weights of less than 2^-39 of the
+    the digits that it is cut into (2^-18); the same but the last two again in the denominator. Weights of less than 2^-41 of the
     largest may lose 2^-13 of an output together. Sums of `steps` steps of a warp in numerator (three additions each) and denominator
     (four), and 64 roundings of the warps' and parts' joins and the division."""
     x, g = np.abs(s).max() / math.log(2), (s.max() - s.min()) / math.log(2) + v_octaves
-    return 2 * math.log(2) * 2.0 ** -24 * (5 * x + g + 31) + 2 * 2.0 ** -22 + 2.0 ** -24 + 2.0 ** -18 + (2.0 ** -13 if g >= 39 else 0) + (7 * steps + 64) * 2.0 ** -24
+    return 2 * math.log(2) * 2.0 ** -24 * (5 * x + g + 31) + 2 * 2.0 ** -22 + 2.0 ** -24 + 2.0 ** -18 + (2.0 ** -13 if g >= 41 else 0) + (7 * steps + 64) * 2.0 ** -24
 
 
 def _check_elements(a, v_octaves, steps, rows=None):
@@ -51,9 +53,9 @@ def _check_elements(a, v_octaves, steps, rows=None):
     worst = 0.0
     for r in range(a.rows) if rows is None else rows:
         for h in range(a.heads):
-            s, want, size = _terms(a, r, h)
+            s, want, size, beyond = _terms(a, r, h)
             far = np.abs(got[r, h * a.d:(h + 1) * a.d] - want)
-            tol = _tolerance(s, v_octaves, steps) * size + 2.0 ** -149
+            tol = _tolerance(s, v_octaves, steps) * size + beyond + 2.0 ** -149
             assert (far <= tol).all(), (r, h, float(np.max(far / np.maximum(size, 1e-300))), float(_tolerance(s, v_octaves, steps)), float(size.max()))
             worst = max(worst, float(np.max(far / np.maximum(size, 1e-300))))
     return worst
@@ -116,7 +118,7 @@ def test_tokens_far_below_the_largest_in_pages_of_odd_blocks_and_binary16(dev, w
         got = a.out.float().cpu().numpy().astype(np.float64)
         for r in range(3):
             for h in range(8):
-                s, want, size = _terms(a, r, h)
+                s, want, size, _ = _terms(a, r, h)
                 far = np.abs(got[r, h * 128:(h + 1) * 128] - want)  # binary16 rounds each output by 2^-11 of it, or 2^-25
                 assert (far <= (_tolerance(s, 0, 12) + 2.0 ** -11) * size + 2.0 ** -25).all()
 
@@ -133,13 +135,16 @@ def test_a_value_with_a_large_scale_and_one_code_leaves_the_other_elements(dev, 
     _check_elements(a, octaves, 8)
 
 
-def test_values_whose_scales_differ_by_sixty_orders_of_magnitude_between_tokens(dev, ws):
+@pytest.mark.parametrize("seed", [0, 36, 136, 157, 161, 165])
+def test_values_whose_scales_differ_by_sixty_orders_of_magnitude_between_tokens(dev, ws, seed):
+    """Most elements are made up of few tokens; with the later seeds some of tokens further from the largest than exponentials reach."""
+    torch.manual_seed(seed)
     for d, kv_heads in ((64, 2), (128, 2), (96, 1), (192, 1)):
-        a = _Attention(dev, ws, rows=3, heads=4, kv_heads=kv_heads, d=d, block=16, lengths=[1, 40, 333], seed=13)
+        a = _Attention(dev, ws, rows=3, heads=4, kv_heads=kv_heads, d=d, block=16, lengths=[1, 40, 333], seed=13 + seed)
         s = a.p.scales[1]
         s.copy_(torch.exp(torch.rand_like(s) * 138 - 69))
         codes = a.p.codes[1]
-        codes[torch.rand(codes.shape, device="cuda") < 0.7] = 0  # most elements are made up of few tokens
+        codes[torch.rand(codes.shape, device="cuda") < 0.7] = 0
         a.call().launch(_stream())
         _check_elements(a, 200, 4)
 
