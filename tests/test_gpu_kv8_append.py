@@ -70,3 +70,30 @@ def test_scales_of_every_size_are_rounded_once(dev):
     _append(p, x, -x, slot_map)
     got_codes, got_scales = p.host()
     assert np.array_equal(got_codes, codes) and np.array_equal(got_scales.astype(np.float32), scales.astype(np.float32))
+
+
+@pytest.mark.parametrize("d,heads,block,tokens,gap", [(64, 2, 16, 1, 0), (96, 3, 5, 33, 1), (128, 8, 16, 300, 2), (192, 2, 32, 65, 3), (256, 1, 16, 40, 5), (128, 5, 64, 700, 7)])
+def test_append_writes_its_places_and_nothing_else(dev, d, heads, block, tokens, gap):
+    """All memory of codes and of scales, between blocks and behind them too, bit for bit."""
+    rng = np.random.default_rng(tokens)
+    p = _Pages(dev, -(-tokens // block) + 3, block, heads, d, seed=tokens, gap=gap)
+    want, want_scales = p.raw.clone(), p.raw_scales.clone()
+    codes, scales = p.host()
+    k, v = (rng.standard_normal((tokens, heads, d)).astype(np.float32) for _ in range(2))
+    slot_map = rng.permutation(p.shape[0] * block)[:tokens].astype(np.int64)
+    slot_map[:tokens // 4] = -1
+    ref.append_ref(codes, scales, k, v, slot_map, tokens)
+    want.as_strided(p.codes.shape, p.codes.stride(), p.codes.storage_offset()).copy_(_up(codes))
+    want_scales.as_strided(p.scales.shape, p.scales.stride(), p.scales.storage_offset()).copy_(_up(scales.astype(np.float32)))
+    _append(p, k, v, slot_map)
+    assert torch.equal(p.raw, want) and torch.equal(p.raw_scales, want_scales)
+
+
+@pytest.mark.parametrize("count", [0, -5, -2 ** 31])
+def test_append_of_no_tokens_writes_nothing(dev, count):
+    p = _Pages(dev, 4, 16, 2, 128, seed=3)
+    codes, scales = p.raw.clone(), p.raw_scales.clone()
+    k, m, n = torch.ones((8, 2, 128), device="cuda"), torch.arange(8, device="cuda"), torch.tensor([count], dtype=torch.int32, device="cuda")
+    jl.Kv8Append(p.pages, k.data_ptr(), k.data_ptr(), GGMLType.F32, tokens=8, slotMap=m.data_ptr(), tokenCount=n.data_ptr()).launch(_stream())
+    torch.cuda.synchronize()
+    assert torch.equal(p.raw, codes) and torch.equal(p.raw_scales, scales)
