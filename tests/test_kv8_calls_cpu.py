@@ -1,10 +1,13 @@
 """The Python calls of the 8-bit paged cache without a GPU, beside tests/test_kv8_cpu.py."""
+import re
+from pathlib import Path
 from types import SimpleNamespace
 
 import pytest
 
 import jitllm_b200 as jl
-from tests.test_kv8_cpu import lib  # noqa: F401
+from tests.test_kernel_source_rules import CSRC, _code, _function_at
+from tests.test_kv8_cpu import ATTENTION, _args, _check, lib  # noqa: F401
 
 AT = 1 << 20
 
@@ -45,3 +48,34 @@ def test_numbers_that_fit_arrive(lib, name, changes):  # noqa: F811
     args = _calls(lib, name, **changes)
     for key, value in changes.items():
         assert getattr(args, {"tokenCount": "token_count"}.get(key, key)) == value
+
+
+def test_the_largest_number_of_rows(lib):  # noqa: F811
+    assert _check(lib, ATTENTION, _args(ATTENTION, rows=1 << 16)) == (0, "")
+    rc, message = _check(lib, ATTENTION, _args(ATTENTION, rows=(1 << 16) + 1))
+    assert rc == 1 and "rows" in message
+
+
+def test_bytes_of_a_block_of_pages(lib):  # noqa: F811
+    """Codes and scales of keys and values, as KvStorage.bytesPerBlock() of the model's own store; gaps between blocks are the caller's."""
+    pages = _pages(SimpleNamespace(_lib=lib), blockStride=8 * 16 * 128 + 64, scaleStride=200)
+    assert pages.bytesPerBlock() == 2 * 8 * 16 * (128 + 4)
+
+
+@pytest.mark.parametrize("name,kernels", [("kv8.cu", 2), ("kv8_attention.cu", 1)])
+def test_in_front_of_the_wait_there_are_declarations_only(name, kernels):
+    """A kernel that is launched while the one ahead still runs may not touch memory before pdl_wait(): what stands in front of it are types,
+    shared arrays, and numbers made of the thread's and the block's indexes and of the parameters."""
+    text = _code(Path(CSRC) / name)
+    found = 0
+    for m in re.finditer(r"__global__", text):
+        body = _function_at(text, m.start())
+        in_front = body[body.index("{") + 1:body.index("pdl_wait()")]
+        found += 1
+        for statement in (x.strip() for x in in_front.split(";")):
+            statement = " ".join(statement.split())
+            assert (re.fullmatch(r"(using .*|constexpr [\w ]+ = .*|pdl_launch_dependents\(\)|)", statement)
+                    or re.fullmatch(r"(extern )?__shared__ [^=]*", statement)
+                    or re.fullmatch(r"const \w+ &a = p\.a", statement)
+                    or re.fullmatch(r"const (int|uint32_t) (\w+ = [\w.%<>&+\- ]+(, )?)+", statement)), statement
+    assert found == kernels
