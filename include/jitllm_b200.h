@@ -365,7 +365,7 @@ int32_t jl_kv8_append(jl_ctx *ctx, const jl_kv8_append_args *args, void *stream)
  * *token_count on are left as they are. A NaN scale, query or key makes NaN of the outputs that it has weight in. Scores and sums are
  * binary32 (scale times a query times codes has to be finite in it); a token's softmax weight times its scale is taken to 2^-18 of
  * itself where it is within 2^-41 of the largest of its sequence; smaller ones lose 2^-13 of an output together at most, and those
- * below 2^-150 of the largest count as 0. */
+ * below 2^-120 of the largest count as 0. */
 typedef struct {
     jl_kv8_pages pages;
     const void *q;                  /* [rows], 16-byte aligned, row stride in elements a multiple of 16 bytes */

@@ -17,7 +17,7 @@
 // What small weights keep. A token far above the others says nothing about an element where its code is 0; that is made up of the
 // others, whose weights must not drown in the digits of the large one. A warp's largest weight times scale is above 2^26, so one within
 // 2^-41 of it (28 nats) is off by 2^-18 of itself at most. What the smaller ones lose is added up, and where it could be more than 2^-13 of an
-// output, the warp goes over its tokens again for the digits behind those (exponentials end at 2^-126, 150 octaves below). Four bytes alone, which lose a weight of 2^-28 of the
+// output, the warp goes over its tokens again for the digits behind those (exponentials end at 2^-126, 120 octaves below or more). Four bytes alone, which lose a weight of 2^-28 of the
 // largest, took (us) 191 for 16 rows at 32000, 11.3 for one row at 3901, 12.9 for 32 rows at 512, 18.9 for 64 rows with a window of 1000; these take
 // 207, 11.5, 13.6 and 21.6. A second pass doubles a warp's time; with scores of 3 nats some warp of a large grid has one in one call of three or so.
 //
@@ -496,7 +496,7 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
             *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + out_at) = x;
         }
         if (a.lse && f % L::kQuads == 0 && g == 0)
-            a.lse[int64_t(row) * a.heads + kv * p.group + head0 + head] = sum == 0.f ? -CUDART_INF_F : (top + __log2f(sum)) * kLn2;
+            a.lse[int64_t(row) * a.heads + kv * p.group + head0 + head] = sum == 0.f ? -CUDART_INF_F : fmaf(top, kLn2, logf(sum));
     };
 
     begin();
@@ -631,11 +631,11 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
             const unsigned mask = *reinterpret_cast<const unsigned *>(stage + L::kMask) >> g;
             const float *ks = reinterpret_cast<const float *>(stage + L::kScales) + g, *vs = ks + kStep;
             float v[4];
-            bool odd_scale = false;  // beyond 2^-60 .. 2^26: exponents are taken apart below, so that no exponential is lost in front of a large scale
+            bool odd_scale = false;  // beyond 2^-60 .. 2^4: exponents are taken apart below, so that no exponential is lost in front of a large scale
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 v[k] = mask >> (8 * k) & 1 ? vs[8 * k] : 1.f;
-                odd_scale = odd_scale || (__float_as_uint(v[k]) & 0x7fffffffu) - 0x21800000u > 0x4c800000u - 0x21800000u;
+                odd_scale = odd_scale || (__float_as_uint(v[k]) & 0x7fffffffu) - 0x21800000u > 0x41800000u - 0x21800000u;
             }
             float y[NT][4], keep[NT];
             float least = kDeep;  // of the weights
@@ -651,7 +651,8 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
                     const int at2 = 2 * (k & 1);
                     const float dot = fmaf(float(c[0][at2] * 256 + c[0][at2 + 1]), 65536.f, float(c[1][at2] * 256 + c[1][at2 + 1]));
                     x[k] = mask >> (8 * k) & 1 ? dot * factor[n] * ks[8 * k] : -CUDART_INF_F;
-                    y[n][k] = exp2_approx(x[k] - e[n]) * v[k];
+                    // from the largest's place, not from the unit's, which is 26 octaves away: the difference would be rounded 2^5 times as coarsely
+                    y[n][k] = exp2_approx(x[k] - (e[n] + kHeadroom)) * (v[k] * 0x1p26f);
                     beyond = beyond || x[k] - m[n] > 20.f || fabsf(y[n][k]) > 1.5e9f;
                 }
                 if (__any_sync(~0u, beyond)) {
@@ -676,7 +677,7 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
                     m[n] = m_new;
                     e[n] = e_new;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) y[n][k] = exp2_approx(x[k] - e[n] + exponent[k]) * mantissa[k];
+                    for (int k = 0; k < 4; ++k) y[n][k] = exp2_approx(x[k] - (e[n] + kHeadroom) + exponent[k]) * (mantissa[k] * 0x1p26f);
                 }
 #pragma unroll
                 for (int k = 0; k < 4; ++k) l[n] += exp2_approx(x[k] - m[n]);
