@@ -567,8 +567,8 @@ __global__ void __launch_bounds__((Shape<HD, NT>::kThreads), (Shape<HD, NT>::kRe
 #pragma unroll
         for (int n = 0; n < NT; ++n) factor[n] = s_scale[4 * n + t];
 
-        // ---- one pass over this warp's tokens: lane (g, t) has tokens g, g + 8, g + 16, g + 24 of a step, heads 4 n + t, elements of
-        // column g. The four tokens of g are bytes of one word of weights, and so are those of t and of t + 4 in a word of values.
+        // ---- one pass over this warp's tokens, or more where small weights want it: lane (g, t) has tokens g, g + 8, g + 16, g + 24 of a
+        // step, heads 4 n + t, elements of column g. The four tokens of g are bytes of one word of weights, and so are those of t and of t + 4 in a word of values.
         float m[NT], e[NT], l[NT], o[NT][L::kQuads][4];
         int acc[NT][2 * L::kQuads][4];  // elements 2 i and 2 i + 1 of a word; bytes 7 and 6 of the weights
         float loss[NT];                 // of weights below kLow
